@@ -65,6 +65,31 @@ class Block(ctypes.Structure):
                 + [(n, c_int) for n in ("B", "S", "H", "hq", "hkv", "D", "E", "I", "I_s", "bn", "bn_s")])
 
 
+class Paged(ctypes.Structure):
+    """cd_paged of include/cdeep.h."""
+    _fields_ = ([("k", c_void_p), ("v", c_void_p)] + [(n, c_longlong) for n in ("stride_p", "stride_h", "stride_t")]
+                + [("table", c_void_p), ("table_stride", c_longlong), ("lengths", c_void_p), ("weights", c_void_p)]
+                + [(n, c_int) for n in ("pages", "page", "width")])
+
+
+class PagedStep(ctypes.Structure):
+    """cd_paged_step of include/cdeep.h."""
+    _fields_ = ([(n, c_void_p) for n in ("q_w", "k_w", "cos_t", "sin_t", "positions", "row_positions")]
+                + [("eps", c_float), ("table_rows", c_int)])
+
+
+class Evict(ctypes.Structure):
+    """cd_evict of include/cdeep.h."""
+    _fields_ = ([(n, c_void_p) for n in ("positions", "row_positions", "weights_out", "row_positions_out")]
+                + [("keep", c_int), ("recent", c_int)])
+
+
+class Sample(ctypes.Structure):
+    """cd_sample of include/cdeep.h."""
+    _fields_ = ([(n, c_void_p) for n in ("uniform", "temperatures", "top_ps", "min_ps", "top_ks")]
+                + [(n, c_float) for n in ("temperature", "top_p", "min_p")] + [("top_k", c_int)])
+
+
 _WINDOW_FN = (c_int, [ctypes.POINTER(WindowAttn), c_int, c_void_p])
 _LATENT_FN = (c_int, [ctypes.POINTER(LatentAttn), c_int, c_void_p])
 _DELTA_FN = (c_int, [ctypes.POINTER(DeltaAttn), c_int, c_void_p])
@@ -199,6 +224,16 @@ SIGNATURES = {
     "cd_gather_div": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_void_p]),
     "cd_combine_top": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p]),
     "cd_gla_chunk": (c_int, [ctypes.POINTER(LinearAttn), c_void_p, c_size_t, c_void_p]),
+    "cd_paged_attention_workspace_bytes": (c_size_t, [c_int] * 7),
+    "cd_paged_attention": (c_int, [ctypes.POINTER(Paged), c_void_p, c_longlong, c_float, c_int, c_int, c_int, c_int, c_void_p,
+                                   c_void_p, c_size_t, c_void_p]),
+    "cd_paged_step_attention": (c_int, [ctypes.POINTER(Paged), ctypes.POINTER(PagedStep), c_void_p, c_float, c_int, c_int, c_int,
+                                        c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cd_evict_rows_workspace_bytes": (c_size_t, [c_int] * 6),
+    "cd_evict_rows": (c_int, [ctypes.POINTER(Paged), ctypes.POINTER(Evict), c_int, c_longlong, c_int, c_int, c_int, c_void_p,
+                              c_size_t, c_void_p]),
+    "cd_sample_tokens": (c_int, [c_void_p, c_int, c_longlong, c_int, c_int, ctypes.POINTER(Sample), c_void_p, c_void_p,
+                                 c_void_p]),
 }
 
 _lib = None

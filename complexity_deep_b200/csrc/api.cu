@@ -30,7 +30,7 @@ const char* cd_error_string(int status) {
     case CD_ERR_CUDA: return "CUDA call failed";
     case CD_ERR_UNSUPPORTED: return "unsupported shape";
     case CD_ERR_TIMEOUT: return "a kernel gave up on a bounded wait";
-    case CD_ERR_BOUNDS: return "checking build: a kernel met an index, address or segment table out of range";
+    case CD_ERR_BOUNDS: return "checking build or paged cache: a kernel met an index, address or segment table out of range";
     default: return "unknown status";
   }
 }
@@ -1005,6 +1005,84 @@ int cd_combine_top(const void* y, const int32_t* inv_perm, const float* weights,
     return CD_ERR_INVALID;
   cudaError_t e = launch_combine_top(y, inv_perm, weights, top, scale, stream_rows, T, ldx, fp32, as_stream(stream));
   return e == cudaSuccess ? CD_OK : cuda_fail(e, "combine_top launch");
+}
+
+// ------------------------------------------------------------------ paged cache, sampling
+static int paged_args_ok(const cd_paged* c, int B, int hkv, int D) {
+  if (!c || B < 1 || hkv < 1 || D < 1) return CD_ERR_INVALID;
+  if (!c->k || !c->v || !c->table || !c->lengths || !aligned16(c->k) || !aligned16(c->v)) return CD_ERR_INVALID;
+  if (c->pages < 1 || c->page < 1 || c->width < 1 || c->table_stride < 0) return CD_ERR_INVALID;
+  if (c->stride_p < 0 || c->stride_h < 0 || c->stride_t < 0 || ((c->stride_p | c->stride_h | c->stride_t | D) & 7)) return CD_ERR_INVALID;
+  if (static_cast<long long>(c->width) * c->page > 0x7fffffffLL - 1024) return CD_ERR_UNSUPPORTED;   // row numbers are 32-bit
+  return CD_OK;
+}
+
+static int paged_shape_ok(int hq, int hkv, int D, int page) {
+  if (hq < 1 || hkv < 1 || hq % hkv) return CD_ERR_INVALID;
+  if ((D != 64 && D != 128) || hq / hkv > 16) return CD_ERR_UNSUPPORTED;
+  return page == 16 || page == 32 || page == 64 || page == 128 || page == 256 ? CD_OK : CD_ERR_UNSUPPORTED;
+}
+
+size_t cd_paged_attention_workspace_bytes(int B, int hq, int hkv, int D, int page, int width, int weights) {
+  if (B < 1 || width < 1 || paged_shape_ok(hq, hkv, D, page) != CD_OK) return 0;
+  return paged_attention_workspace_bytes(B, hq, hkv, D, page, width, weights != 0);
+}
+
+static int paged_attention(const cd_paged* c, const cd_paged_step* step, const void* q, long long q_stride, float scale, int B, int hq,
+                           int hkv, int D, void* out, void* ws, size_t ws_bytes, void* stream) {
+  int st = paged_args_ok(c, B, hkv, D);
+  if (st == CD_OK) st = paged_shape_ok(hq, hkv, D, c->page);
+  if (st != CD_OK) return st;
+  if (!q || !out || !aligned16(q) || !aligned16(out) || (q_stride & 7) || q_stride < 0) return CD_ERR_INVALID;
+  const size_t need = paged_attention_workspace_bytes(B, hq, hkv, D, c->page, c->width, c->weights != nullptr);
+  if (need && (!ws || !aligned16(ws) || ws_bytes < need)) return CD_ERR_INVALID;
+  if (B > 65535) return CD_ERR_UNSUPPORTED;
+  int* status = device_status_word();
+  if (!status) return CD_ERR_CUDA;
+  const cudaError_t e = launch_paged_attention(*c, step, q, q_stride, scale, B, hq, hkv, D, out, ws, status, as_stream(stream));
+  return e == cudaSuccess ? CD_OK : cuda_fail(e, "paged attention launch");
+}
+
+int cd_paged_attention(const cd_paged* c, const void* q, long long q_stride_b, float scale, int B, int hq, int hkv, int D, void* out,
+                       void* ws, size_t ws_bytes, void* stream) {
+  return paged_attention(c, nullptr, q, q_stride_b, scale, B, hq, hkv, D, out, ws, ws_bytes, stream);
+}
+
+int cd_paged_step_attention(const cd_paged* c, const cd_paged_step* step, const void* qkv, float scale, int B, int hq, int hkv, int D,
+                            void* out, void* ws, size_t ws_bytes, void* stream) {
+  if (!step || !step->cos_t || !step->sin_t || !step->positions || step->table_rows < 1) return CD_ERR_INVALID;
+  if ((step->q_w == nullptr) != (step->k_w == nullptr)) return CD_ERR_INVALID;
+  return paged_attention(c, step, qkv, static_cast<long long>(hq + 2LL * hkv) * D, scale, B, hq, hkv, D, out, ws, ws_bytes, stream);
+}
+
+size_t cd_evict_rows_workspace_bytes(int layers, int B, int hkv, int page, int width, int keep) {
+  if (layers < 1 || B < 1 || hkv < 1 || page < 1 || width < 1 || keep < 1) return 0;
+  return evict_rows_workspace_bytes(layers, B, hkv, page, width, keep);
+}
+
+int cd_evict_rows(const cd_paged* c, const cd_evict* e, int layers, long long stride_l, int B, int hkv, int D, void* ws, size_t ws_bytes,
+                  void* stream) {
+  const int st = paged_args_ok(c, B, hkv, D);
+  if (st != CD_OK) return st;
+  if (!e || layers < 1 || (stride_l & 7) || stride_l < 0 || !c->weights || !e->positions || !e->row_positions || !e->weights_out ||
+      !e->row_positions_out || e->keep < 1 || e->recent < 0 || e->recent > e->keep)
+    return CD_ERR_INVALID;
+  if ((e->weights_out == c->weights) != (e->row_positions_out == e->row_positions)) return CD_ERR_INVALID;
+  if (static_cast<long long>(layers) * B * hkv > 0x7fffffffLL / 16) return CD_ERR_UNSUPPORTED;
+  const size_t need = evict_rows_workspace_bytes(layers, B, hkv, c->page, c->width, e->keep);
+  if (need && (!ws || !aligned16(ws) || ws_bytes < need)) return CD_ERR_INVALID;
+  int* status = device_status_word();
+  if (!status) return CD_ERR_CUDA;
+  const cudaError_t err = launch_evict_rows(*c, *e, layers, stride_l, B, hkv, D, ws, status, as_stream(stream));
+  return err == cudaSuccess ? CD_OK : cuda_fail(err, "evict rows launch");
+}
+
+int cd_sample_tokens(const void* logits, int fp32, long long ld, int B, int V, const cd_sample* p, int64_t* ids, float* probs,
+                     void* stream) {
+  if (!logits || !p || !p->uniform || !ids || !probs || B < 1 || V < 1 || ld < V) return CD_ERR_INVALID;
+  if (V > (1 << 18)) return CD_ERR_UNSUPPORTED;                    // masses are sums of 2^18 numbers up to 2^44
+  const cudaError_t e = launch_sample_tokens(logits, fp32 ? 1 : 0, ld, B, V, *p, ids, probs, as_stream(stream));
+  return e == cudaSuccess ? CD_OK : cuda_fail(e, "sample tokens launch");
 }
 
 }  // extern "C"

@@ -15,7 +15,7 @@ constexpr bool kChecks = false;
 
 constexpr int kStatusWaitTimeout = 1;   // a bounded pipeline wait ran out
 constexpr int kStatusPeerTimeout = 2;   // the barrier between GPUs ran out
-constexpr int kStatusBounds = 4;        // checking build: an index / address / segment table was invalid
+constexpr int kStatusBounds = 4;        // checking build, and paged caches always: an index / address / segment table was invalid
 
 // true when 0 <= v < n (always true in the normal build)
 __device__ __forceinline__ bool index_ok(int v, int n, int* status) {

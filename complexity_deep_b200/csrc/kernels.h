@@ -244,4 +244,14 @@ int* device_status_word();  // per-device word the kernels raise when a bounded 
 extern thread_local char g_cuda_err[256];        // text behind cd_last_cuda_error()
 int cuda_fail(cudaError_t e, const char* what);  // records the text, returns CD_ERR_CUDA
 
+// paged cache (paged_attention.cu, evict_rows.cu) and sampling (sample_tokens.cu)
+size_t paged_attention_workspace_bytes(int B, int hq, int hkv, int D, int page, int width, bool weights);
+cudaError_t launch_paged_attention(const cd_paged& c, const cd_paged_step* step, const void* q, long long q_stride, float scale, int B,
+                                   int hq, int hkv, int D, void* out, void* ws, int* status, cudaStream_t stream);
+size_t evict_rows_workspace_bytes(int layers, int B, int hkv, int page, int width, int keep);
+cudaError_t launch_evict_rows(const cd_paged& c, const cd_evict& e, int layers, long long stride_l, int B, int hkv, int D, void* ws,
+                              int* status, cudaStream_t stream);
+cudaError_t launch_sample_tokens(const void* logits, int fp32, long long ld, int B, int V, const cd_sample& p, int64_t* ids, float* probs,
+                                 cudaStream_t stream);
+
 }  // namespace cdeep

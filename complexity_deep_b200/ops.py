@@ -111,8 +111,8 @@ def status_fetch() -> int:
     st = ctypes.c_int(0)
     _lib.check(lib.cd_status_fetch(ctypes.byref(st)), "cd_status_fetch")
     if st.value == 4:
-        raise _lib.CdeepError("checking build: a libcdeep kernel met an index, address or segment "
-                              "table out of range and skipped the access")
+        raise _lib.CdeepError("a libcdeep kernel met an index, address or segment table out of range and skipped the "
+                              "access (page tables, lengths and positions of a paged cache; checking build: row maps too)")
     if st.value != 0:
         raise _lib.CdeepError("a libcdeep kernel gave up on a bounded wait (pipeline error)")
     return st.value
@@ -1392,3 +1392,187 @@ def combine_top_(stream: torch.Tensor, y: torch.Tensor, inv_perm: torch.Tensor, 
         _lib.check(lib.cd_combine_top(y.data_ptr(), inv_perm.data_ptr(), weights.data_ptr(), top, float(scale),
                                       stream.data_ptr(), T, stream.shape[1], fp32, _stream()), "cd_combine_top")
     return stream
+
+
+# --------------------------------------------------------------------------- paged cache
+def _on(t: torch.Tensor, name: str, dtype, device, shape) -> int:
+    """Address of a contiguous tensor of that type, device and shape."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or tuple(t.shape) != shape:
+        raise RuntimeError(f"{name}: expected a {dtype} tensor of shape {list(shape)} on {device}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous tensor")
+    return t.data_ptr()
+
+
+def _here(t: torch.Tensor, name: str):
+    """Device of a CUDA tensor, which has to be the current one: launches go to its current stream."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a CUDA tensor; the complexity_deep_b200 kernels have no CPU path")
+    if t.device.index != _current_device():
+        raise RuntimeError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
+    return t.device
+
+
+def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+           weights: Optional[torch.Tensor], layers: int, batch: int, device) -> _lib.Paged:
+    """The cache as the library takes it; pools [pages, kv heads, page, D], of several layers with the layers in front."""
+    shape, strides = k_pages.shape, k_pages.stride()
+    for t, name in ((k_pages, "k pages"), (v_pages, "v pages")):
+        if t.dtype is not BF16 or t.device != device or t.dim() < 4 or t.stride(-1) != 1:
+            raise RuntimeError(f"{name}: expected bf16 [pages, kv heads, page, D] on {device}, D contiguous")
+    if v_pages.shape != shape or v_pages.stride() != strides:
+        raise RuntimeError("k and v pages must share their shape and strides")
+    if any(n % 8 for n in strides[:-1]) or (k_pages.data_ptr() | v_pages.data_ptr()) & 15:
+        raise RuntimeError("pages: strides must be multiples of 8 elements, the pools lie on 16-byte boundaries")
+    if (block_table.dtype is not torch.int32 or block_table.device != device or block_table.dim() != 2
+            or block_table.shape[0] != batch or block_table.shape[1] < 1 or block_table.stride(1) != 1):
+        raise RuntimeError(f"block_table: expected int32 [{batch}, pages of a sequence] on {device}")
+    pages, hkv, page, _ = shape[-4:]
+    width = block_table.shape[1]
+    statistics = (layers, batch, hkv, width * page) if len(shape) == 5 else (batch, hkv, width * page)
+    return _lib.Paged(k_pages.data_ptr(), v_pages.data_ptr(), strides[-4], strides[-3], strides[-2], block_table.data_ptr(),
+                      block_table.stride(0), _on(lengths, "lengths", torch.int32, device, (batch,)),
+                      None if weights is None else _on(weights, "weights", torch.float32, device, statistics), pages, page, width)
+
+
+def _attend_paged(step, c: _lib.Paged, q: torch.Tensor, hq: int, hkv: int, D: int) -> torch.Tensor:
+    lib = _lib.load()
+    B, device = q.shape[0], q.device
+    out = torch.empty(B, hq * D, dtype=BF16, device=device)
+    n = lib.cd_paged_attention_workspace_bytes(B, hq, hkv, D, c.page, c.width, 0 if c.weights is None else 1)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    with _Span("paged_attention"):
+        if step is None:
+            _lib.check(lib.cd_paged_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), D ** -0.5, B, hq, hkv, D, out.data_ptr(),
+                                              _ptr(ws), n, _stream()), "cd_paged_attention")
+        else:
+            _lib.check(lib.cd_paged_step_attention(ctypes.byref(c), ctypes.byref(step), q.data_ptr(), D ** -0.5, B, hq, hkv, D,
+                                                   out.data_ptr(), _ptr(ws), n, _stream()), "cd_paged_step_attention")
+    return out
+
+
+def _heads(k_pages: torch.Tensor, hq: int, hkv: int, head_dim: int) -> None:
+    if head_dim not in (64, 128) or hkv < 1 or hq < 1 or hq % hkv or hq // hkv > 16:
+        raise RuntimeError("paged attention needs head size 64 or 128 and at most 16 query heads per KV head")
+    if k_pages.dim() != 4 or k_pages.shape[1] != hkv or k_pages.shape[3] != head_dim or k_pages.shape[2] not in (16, 32, 64, 128, 256):
+        raise RuntimeError(f"pages: expected [pages, {hkv}, 16 / 32 / 64 / 128 / 256 rows, {head_dim}]")
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    lengths: torch.Tensor, hq: int, hkv: int, head_dim: int,
+                    weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query per sequence over a paged cache.  q [B, at least hq * D] (its first columns are used: the fused projection
+    buffer will do), pages [pages, hkv, page, D] of any strides, block_table int32 [B, width] (row r of a sequence is in page
+    ``block_table[b, r // page]``), lengths int32 [B] on the device (0 or less: the output row is zeros).  `weights` (fp32
+    [B, hkv, width * page]): every row's softmax weight, summed over the query heads of its KV head, is added there.
+    Returns [B, hq * D].  A page outside the pool raises in ``status_fetch``."""
+    device = _here(q, "q")
+    _heads(k_pages, hq, hkv, head_dim)
+    if q.dtype is not BF16 or q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < hq * head_dim or q.stride(0) % 8 or q.data_ptr() & 15:
+        raise RuntimeError("q: expected bf16 rows of at least hq * head_dim elements on 16-byte boundaries")
+    forward_only(q, "paged_attention")
+    c = _paged(k_pages, v_pages, block_table, lengths, weights, 1, q.shape[0], device)
+    return _attend_paged(None, c, q, hq, hkv, head_dim)
+
+
+def paged_step_attention(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor], cos: torch.Tensor,
+                         sin: torch.Tensor, eps: float, hq: int, hkv: int, head_dim: int, k_pages: torch.Tensor,
+                         v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,
+                         weights: Optional[torch.Tensor] = None, row_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A decode step on a paged cache in one call: Q/K RMSNorm and rotation of qkv [B, (hq + 2 hkv) * D] at positions[b], the
+    new key and value stored as row lengths[b], then ``paged_attention`` over lengths[b] + 1 rows.  qkv, lengths and positions
+    stay as they are (all layers of a model use them).  The new row's entry of `weights` starts from its own weight, that of
+    `row_positions` (int32, same shape) becomes positions[b].  lengths[b] < 0 marks a slot that is not in use: its output is
+    zeros and nothing is stored.  A sequence without room for the row, and a position without a rotation, is treated the
+    same way and raises in ``status_fetch``.  Returns [B, hq * D]."""
+    device = _here(qkv, "qkv")
+    _heads(k_pages, hq, hkv, head_dim)
+    B, D = qkv.shape[0], head_dim
+    forward_only(qkv, "paged_step_attention")
+    if (q_w is None) != (k_w is None):
+        raise RuntimeError("norm weights: both or none")
+    c = _paged(k_pages, v_pages, block_table, lengths, weights, 1, B, device)
+    rows = c.width * c.page
+    if cos.dim() != 2:
+        raise RuntimeError("cos/sin: expected [positions, head_dim]")
+    table = (cos.shape[0], D)
+    step = _lib.PagedStep(
+        None if q_w is None else _on(q_w, "q_norm.weight", BF16, device, (D,)),
+        None if k_w is None else _on(k_w, "k_norm.weight", BF16, device, (D,)),
+        _on(cos, "cos", torch.float32, device, table), _on(sin, "sin", torch.float32, device, table),
+        _on(positions, "positions", torch.int32, device, (B,)),
+        None if row_positions is None else _on(row_positions, "row_positions", torch.int32, device, (B, hkv, rows)),
+        float(eps), cos.shape[0])
+    _on(qkv, "qkv", BF16, device, (B, (hq + 2 * hkv) * D))
+    return _attend_paged(step, c, qkv, hq, hkv, D)
+
+
+def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                positions: torch.Tensor, weights: torch.Tensor, row_positions: torch.Tensor, keep: int, recent: int,
+                weights_out: Optional[torch.Tensor] = None, row_positions_out: Optional[torch.Tensor] = None) -> None:
+    """Cuts a paged cache back, in place, to `keep` rows per sequence and KV head: the rows of the last `recent` positions
+    (``row_positions >= positions - recent``) stay first (all alike), then those of largest weight, ties by the lowest row.  Of the rows
+    that stay, the i-th behind row `keep` moves into the place of the i-th given up in front of it; weights and row_positions
+    move along, or the first `keep` rows of both go to the given outputs.  Sequences of at most `keep` rows stay as they are.
+    `lengths` is not changed: the caller cuts it back once every layer is done.  Pools [pages, hkv, page, D] with weights
+    [B, hkv, width * page], or [layers, pages, hkv, page, D] with [layers, B, hkv, width * page].  No page may belong to two
+    sequences."""
+    device = _here(k_pages, "k pages")
+    if k_pages.dim() not in (4, 5):
+        raise RuntimeError("pages: expected [pages, kv heads, page, D] or [layers, pages, kv heads, page, D]")
+    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
+    hkv, D = k_pages.shape[-3], k_pages.shape[-1]
+    keep, recent = int(keep), int(recent)
+    if keep < 1 or not 0 <= recent <= keep:
+        raise RuntimeError("evict_rows_: expected keep >= 1 and 0 <= recent <= keep")
+    if D % 8:
+        raise RuntimeError("pages: the head size must be a multiple of 8")
+    if (weights_out is None) != (row_positions_out is None):
+        raise RuntimeError("evict_rows_: both outputs or none")
+    B = block_table.shape[0]
+    c = _paged(k_pages, v_pages, block_table, lengths, weights, layers, B, device)
+    shape = tuple(weights.shape)
+    if weights_out is None:
+        weights_out, row_positions_out = weights, row_positions
+    e = _lib.Evict(_on(positions, "positions", torch.int32, device, (B,)),
+                   _on(row_positions, "row_positions", torch.int32, device, shape),
+                   _on(weights_out, "weights_out", torch.float32, device, shape),
+                   _on(row_positions_out, "row_positions_out", torch.int32, device, shape), keep, recent)
+    lib = _lib.load()
+    n = lib.cd_evict_rows_workspace_bytes(layers, B, hkv, c.page, c.width, keep)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    with _Span("evict_rows"):
+        _lib.check(lib.cd_evict_rows(ctypes.byref(c), ctypes.byref(e), layers, k_pages.stride(0) if k_pages.dim() == 5 else 0, B, hkv, D,
+                                     _ptr(ws), n, _stream()), "cd_evict_rows")
+
+
+# --------------------------------------------------------------------------- sampling
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of every row of logits [B, V] (bf16 or fp32, V contiguous) from uniform numbers in [0, 1) (fp32 [B]):
+    (ids int64 [B], their probability fp32 [B] among the tokens that stayed).  With w = exp((x - max) / temperature): top_k keeps
+    values at least the k-th largest (ties stay, as in ``sample_next``), top_p what has at most top_p of the remaining mass ahead
+    of it in descending order (ties: lowest index first), min_p what has w >= min_p; the id is the first i, in the order of the
+    vocabulary, with sum_{j <= i} w_j > uniform * sum_j w_j.  Every rule is a number, or a tensor with one entry per row (fp32,
+    top_k int32).  temperature 0 takes the first largest value; top_k 0, top_p 1 and min_p 0 are off.  A NaN is never drawn; a row
+    without a value above -inf gives id 0 with probability 0."""
+    device = _here(logits, "logits")
+    if logits.dtype not in (BF16, torch.float32) or logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:
+        raise RuntimeError("logits: expected bf16 or fp32 [B, V], V contiguous")
+    forward_only(logits, "sample_tokens")
+    B, V = logits.shape
+    if V > 1 << 18:
+        raise RuntimeError("sample_tokens: at most 262144 logits a row")
+    r = _lib.Sample(uniform=_on(uniform, "uniform", torch.float32, device, (B,)))
+    for name, rule, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                              ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(rule, torch.Tensor):
+            setattr(r, name + "s", _on(rule, name, dtype, device, (B,)))
+        else:
+            setattr(r, name, rule)
+    ids = torch.empty(B, dtype=torch.int64, device=device)
+    probs = torch.empty(B, dtype=torch.float32, device=device)
+    if B:
+        with _Span("sample_tokens"):
+            _lib.check(_lib.load().cd_sample_tokens(logits.data_ptr(), int(logits.dtype is torch.float32), logits.stride(0), B, V,
+                                                    ctypes.byref(r), ids.data_ptr(), probs.data_ptr(), _stream()), "cd_sample_tokens")
+    return ids, probs

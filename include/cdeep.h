@@ -32,8 +32,8 @@ extern "C" {
 #define CD_ERR_CUDA 2         /* a CUDA runtime / driver call failed; see cd_last_cuda_error */
 #define CD_ERR_UNSUPPORTED 3  /* shape outside what the kernels implement */
 #define CD_ERR_TIMEOUT 4      /* a kernel gave up on a bounded wait (reported by cd_status_fetch) */
-#define CD_ERR_BOUNDS 5       /* checking build only: an index / address / segment table read from device
-                                 memory was out of range (reported by cd_status_fetch) */
+#define CD_ERR_BOUNDS 5       /* checking build, and paged caches in any build: an index / address / segment
+                                 table read from device memory was out of range (reported by cd_status_fetch) */
 
 /* ABI version of this header (bumped on any signature change; currently 4). */
 int cd_version(void);
@@ -664,6 +664,89 @@ int cd_gather_div(const void* x, const int32_t* perm, int div, void* out, int64_
 /* stream[t] += scale * sum_j weights[t, j] * y[inv_perm[t * top + j]]; y [T * top, ldx]. */
 int cd_combine_top(const void* y, const int32_t* inv_perm, const float* weights, int top, float scale,
                    float* stream_rows, int T, int ldx, int fp32, void* stream);
+
+/* ------------------------------------------------------------------ paged cache --------------
+ * Keys and values of sequences of different lengths (no counterpart in the reference): row r of
+ * sequence b lies in page table[b, r / page] at place r % page.  What lengths, tables and positions
+ * hold is read and checked on the device: a page outside [0, pages), a length beyond width * page or
+ * a position without a rotation raises the status word (cd_status_fetch: CD_ERR_BOUNDS) and is not
+ * followed. */
+typedef struct cd_paged {
+  void* k;                  /* bf16 pages [pages, kv heads, page, D] of any strides (elements, */
+  void* v;                  /* multiples of 8; the same for both), D contiguous */
+  long long stride_p, stride_h, stride_t;
+  const int32_t* table;     /* [B, width], rows table_stride apart */
+  long long table_stride;
+  const int32_t* lengths;   /* [B] cached rows */
+  float* weights;           /* [B, kv heads, width * page] accumulated attention weights, or NULL */
+  int pages, page, width;   /* page: 16, 32, 64, 128 or 256 rows */
+} cd_paged;
+
+/* What a decode step brings besides the projections. */
+typedef struct cd_paged_step {
+  const void* q_w;          /* [D] norm weights, or both NULL */
+  const void* k_w;
+  const float* cos_t;       /* [table_rows, D] */
+  const float* sin_t;
+  const int32_t* positions; /* [B] of the new tokens */
+  int32_t* row_positions;   /* [B, kv heads, width * page] position of every cached row, or NULL */
+  float eps;
+  int table_rows;
+} cd_paged_step;
+
+/* One query per sequence over its lengths[b] rows (none: zeros; below 0: the same):
+ *   out[b, h] = softmax(scale q[b, h] . K_b^T) V_b;  weights[b, h / G, r] += sum over the G heads of p[r]
+ * Sequences may share pages.  D is 64 or 128, G = hq / hkv <= 16; q rows q_stride_b elements apart (a
+ * multiple of 8).  ws: cd_paged_attention_workspace_bytes(...) bytes, NULL where that is 0. */
+size_t cd_paged_attention_workspace_bytes(int B, int hq, int hkv, int D, int page, int width, int weights);
+int cd_paged_attention(const cd_paged* h_cache, const void* q, long long q_stride_b, float scale, int B,
+                       int hq, int hkv, int D, void* out, void* ws, size_t ws_bytes, void* stream);
+/* A decode step: qkv [B, (hq + 2 hkv) * D]; q and k heads normalised and rotated at positions[b], k (rounded to
+ * bf16) and v stored as row lengths[b], whose weight starts from 0, then attention over lengths[b] + 1 rows.
+ * qkv and lengths stay as they are.  lengths[b] < 0: the slot is not in use, its output is zeros and nothing is
+ * stored; the same, with the status word, for a sequence without room. */
+int cd_paged_step_attention(const cd_paged* h_cache, const cd_paged_step* h_step, const void* qkv, float scale,
+                            int B, int hq, int hkv, int D, void* out, void* ws, size_t ws_bytes, void* stream);
+
+/* Eviction: what is kept of a paged cache.  weights, row_positions and their outputs
+ * [layers, B, kv heads, width * page]; the outputs may be the inputs. */
+typedef struct cd_evict {
+  const int32_t* positions;     /* [B] position of the next token */
+  const int32_t* row_positions;
+  float* weights_out;
+  int32_t* row_positions_out;
+  int keep, recent;
+} cd_evict;
+
+/* Every (layer, sequence, KV head) with more than `keep` rows is cut back to `keep`: rows at positions from
+ * positions[b] - recent on stay first (all alike), then those of largest weight (NaN above all numbers), ties by
+ * the lowest row.  The i-th row that stays behind row `keep` moves into the place of the i-th one given up in front of it;
+ * rows from `keep` on are left as they are.  lengths is not changed (the layers of a model share it).  Sequences
+ * must not share pages.  Pools of the layers stride_l elements apart; D a multiple of 8, pages of any size. */
+size_t cd_evict_rows_workspace_bytes(int layers, int B, int hkv, int page, int width, int keep);
+int cd_evict_rows(const cd_paged* h_cache, const cd_evict* h_evict, int layers, long long stride_l, int B, int hkv,
+                  int D, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------ sampling -----------------
+ * The next token of every row of logits [B, V] (bf16 or fp32, rows ld elements apart), from given uniform
+ * numbers.  With w = exp((x - max) / temperature): top-k keeps values at least the k-th largest (ties stay),
+ * top-p what has, in descending order (ties: lowest index first), at most top_p of the mass that top-k has left
+ * ahead of it, min-p what has w >= min_p; the id is the first i with sum_{j <= i} w_j > uniform sum_j w_j.
+ * probs: w_id / sum.  temperature <= 0: the first largest value.  top_k <= 0, top_p >= 1, min_p <= 0: off.  A
+ * NaN is never drawn; a row without a value above -inf gives id 0 and probability 0.  V <= 2^18.  Replaces
+ * complexity_deep/models/modeling.py:256-296. */
+typedef struct cd_sample {
+  const float* uniform;         /* [B] in [0, 1) */
+  const float* temperatures;    /* [B] each, or NULL: the number below for all rows */
+  const float* top_ps;
+  const float* min_ps;
+  const int32_t* top_ks;
+  float temperature, top_p, min_p;
+  int top_k;
+} cd_sample;
+
+int cd_sample_tokens(const void* logits, int fp32, long long ld, int B, int V, const cd_sample* h_rules, int64_t* ids,
+                     float* probs, void* stream);
 
 #ifdef __cplusplus
 }
