@@ -1036,7 +1036,7 @@ static int paged_attention(const cd_paged* c, const cd_paged_step* step, const v
   if (!q || !out || !aligned16(q) || !aligned16(out) || (q_stride & 7) || q_stride < 0) return CD_ERR_INVALID;
   const size_t need = paged_attention_workspace_bytes(B, hq, hkv, D, c->page, c->width, c->weights != nullptr);
   if (need && (!ws || !aligned16(ws) || ws_bytes < need)) return CD_ERR_INVALID;
-  if (B > 65535) return CD_ERR_UNSUPPORTED;
+  if ((static_cast<long long>(c->width) * c->page + 63) / 64 * B * hkv > 0x7fffffffLL) return CD_ERR_UNSUPPORTED;   // tiles are counted in 32 bits
   int* status = device_status_word();
   if (!status) return CD_ERR_CUDA;
   const cudaError_t e = launch_paged_attention(*c, step, q, q_stride, scale, B, hq, hkv, D, out, ws, status, as_stream(stream));
@@ -1052,6 +1052,8 @@ int cd_paged_step_attention(const cd_paged* c, const cd_paged_step* step, const 
                             void* out, void* ws, size_t ws_bytes, void* stream) {
   if (!step || !step->cos_t || !step->sin_t || !step->positions || step->table_rows < 1) return CD_ERR_INVALID;
   if ((step->q_w == nullptr) != (step->k_w == nullptr)) return CD_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(step->q_w) & 3) || ((reinterpret_cast<uintptr_t>(step->cos_t) | reinterpret_cast<uintptr_t>(step->sin_t)) & 7))
+    return CD_ERR_INVALID;
   return paged_attention(c, step, qkv, static_cast<long long>(hq + 2LL * hkv) * D, scale, B, hq, hkv, D, out, ws, ws_bytes, stream);
 }
 

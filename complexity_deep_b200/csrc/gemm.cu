@@ -301,6 +301,21 @@ bool encode_map_2d(void* map_out, const void* base, long long rows, long long co
   return make_map(static_cast<CUtensorMap*>(map_out), base, rows, cols, ld, box_rows);
 }
 
+// bf16 tensor [dims[3], dims[2], dims[1], dims[0]] with the given distances in elements (of dims[1], dims[2], dims[3]; the innermost
+// is contiguous); box = [1, 1, box_rows, 64], 128-byte swizzle, zero fill out of bounds.
+bool encode_map_4d(void* map_out, const void* base, const int (&dims)[4], const long long (&strides)[3], int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  cuuint64_t size[4], bytes[3];
+  for (int i = 0; i < 4; ++i) size[i] = static_cast<cuuint64_t>(dims[i]);
+  // nothing is ever as far away as the distance of a dimension of one says
+  for (int i = 0; i < 3; ++i) bytes[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(strides[i]) * 2 : static_cast<cuuint64_t>(dims[0]) * 2;
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(kBoxK), static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
+  return fn(static_cast<CUtensorMap*>(map_out), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), size, bytes, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static DeviceInfo* device_info(int* status_out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

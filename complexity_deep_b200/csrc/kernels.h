@@ -94,6 +94,7 @@ int splitk_config(int flags);   // sets which forms of split-K may be used (nega
 // between rows, boxes of [box_rows, 64 columns], 128-byte swizzle, zero fill out of bounds.
 bool encode_map_2d(void* map_out, const void* base, long long rows, long long cols, long long ld,
                    int box_rows);
+bool encode_map_4d(void* map_out, const void* base, const int (&dims)[4], const long long (&strides)[3], int box_rows);
 
 // causal prefill attention over the fused projection buffer (attention_prefill.cu)
 cudaError_t launch_attention_prefill(const void* qkv, void* out, int B, int S, int hq, int hkv, int D,

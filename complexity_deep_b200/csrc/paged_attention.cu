@@ -3,49 +3,176 @@
 //
 //   s_{g,r} = scale q_g . k_r;  p = exp(s - max) / sum;  out_g = sum_r p_{g,r} v_r;  weights_r += sum_g p_{g,r}
 //
-// for the G query heads g of a KV head. One block a (sequence, KV head): its warps take the rows in turn, a lane D / 32 columns,
-// each with a running maximum and sum, which meet in shared memory. Scores are kept for the accumulator, whose share of a row is
-// known only when maximum and sum are.
+// for the G query heads g of a KV head: every cached row is read once for all of them, so the read (4 D bytes a row and head) is
+// the bound, and G only has to stay out of its way. Hence matrix instructions (m16n8k16): the query heads are the 16 rows of one
+// operand. Up to eight heads leave half of them free, which hold what bf16 cuts off: q and p enter as two bf16 numbers (16
+// significant bits) at no cost. More heads take two products instead.
 //
-// A step (kStep) brings the raw projections: the block normalises and rotates its heads first, writes key and value into the new
-// row's place and takes that row with the others. The query stays in 32 bits.
+// Work is cut into tiles of 64 rows; all tiles of all (sequence, KV head) pairs stand in one line, of which every block takes an equal
+// stretch, whatever the lengths are. A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
+// block, which the second kernel adds in order (results do not depend on timing). A warp feeds tiles to the ring with TMA (a
+// box per page, 128-byte swizzle), four warps take 16 rows of a tile each, with a running maximum and sum of their own.
+//
+// The share of a row in its softmax is known only when the pair's maximum and sum are: where weights are asked for, scores are
+// left in the workspace and the second kernel turns them into shares.
+//
+// A step (kStep) brings the raw projections: a warp normalises and rotates the query heads where it needs them, in the registers that
+// the products take; the block that has the pair's last tile does so for the key, writes key and value into the new row's place, in
+// the cache and in its copy of the tile.
 #include <cfloat>
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "checks.cuh"
-#include "elem.cuh"
 #include "kernels.h"
+#include "mma.cuh"
 #include "ptx.cuh"
 
 namespace cdeep {
 
 namespace {
 
-// warps of a block: their sums of kG heads share its 48 KB
-__host__ __device__ constexpr int warps_of(int kG) { return kG > 8 ? 4 : 8; }
+constexpr int kTile = 64;                 // rows of a tile
+constexpr int kWarps = 4;                 // that compute; one more feeds them
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr float kLog2e = 1.4426950408889634f;
+
+__host__ __device__ constexpr int stage_bytes(int D) { return 2 * kTile * D * 2; }
+// floats of a lane that a warp hands over: its columns of each head it holds
+__host__ __device__ constexpr int lane_floats(int D, bool wide) { return D / 8 * (wide ? 4 : 2); }
+__host__ __device__ constexpr int merge_bytes(int D, bool wide) { return (kWarps - 1) * 32 * (lane_floats(D, wide) + 4) * 4; }
+// Two blocks an SM (113 KB each): one computes while the other starts a pair or ends one. 16 heads of 128 leave room for one.
+__host__ __device__ constexpr int blocks_per_sm(int D, bool wide) { return wide && D == 128 ? 1 : 2; }
+__host__ __device__ constexpr int stages_of(int D, bool wide) {
+  return (232448 / blocks_per_sm(D, wide) - 1024 * 3 - merge_bytes(D, wide)) / stage_bytes(D);
+}
+__host__ __device__ constexpr int smem_bytes(int D, bool wide) {
+  return 1024 + stages_of(D, wide) * stage_bytes(D) + merge_bytes(D, wide);
+}
+
+// What a pair is, for the second kernel.
+struct Pair {
+  int unit;               // its first tile in the line
+  int first, last;        // blocks that have tiles of it; first = -1: none
+  int rows;
+};
 
 struct Args {
   cd_paged c;
   const bf16* q;
   long long q_stride;
   cd_paged_step st;
-  float scale;
-  int G, hq;
+  float scale_log2;
+  int B, hkv, G;
+  int boxes, box_rows;    // pages of a tile, rows of a page that a tile takes
   bf16* out;
-  float* scores;
   int* status;
+  // workspace
+  int* units;             // [1]
+  int* block_pair;        // [blocks] the pair that a block begins with
+  Pair* pairs;            // [B hkv]
+  float* part;            // [blocks][2][G (D + 2)]: of the first pair of a block and of the last
+  int* unit_pair;         // [tiles]           where weights are asked for
+  float2* top_sum;        // [B hkv][G] maximum and sum of pairs that are not cut
+  float* scores;          // [tiles][G][64], times log2 e
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+__device__ __forceinline__ long long first_unit(long long units, int block, int blocks) { return units * block / blocks; }
+__device__ __forceinline__ int block_of(long long unit, long long units, int blocks) {
+  return static_cast<int>(((unit + 1) * blocks - 1) / units);
 }
 
-// RMS norm (w or none) and rotation of a head; lane l holds columns l + 32 i.
+// Rows of a sequence that this call attends to; -1 where table, length or position do not hold.
+template <bool kStep>
+__device__ __forceinline__ int rows_of(const Args& a, int b) {
+  const int n = a.c.lengths[b], limit = a.c.width * a.c.page;
+  if (n < 0) return 0;
+  if constexpr (!kStep) return n <= limit ? n : -1;
+  if (n >= limit) return -1;
+  const int pos = a.st.positions[b], page = a.c.table[b * a.c.table_stride + n / a.c.page];
+  return pos >= 0 && pos < a.st.table_rows && page >= 0 && page < a.c.pages ? n + 1 : -1;
+}
+__device__ __forceinline__ int tiles_of(int rows) { return rows > 0 ? (rows + kTile - 1) / kTile : 0; }
+
+// A block's way along its stretch.
+struct Walk {
+  int b, h, t, rows;
+  long long left;         // tiles of the stretch from here on
+};
+template <bool kStep>
+__device__ __forceinline__ void next_pair(const Args& a, Walk& w, int taken) {
+  w.left -= taken;
+  w.t = 0;
+  if (++w.h < a.hkv) return;
+  w.h = 0;
+  if (w.left <= 0) return;
+  do w.rows = rows_of<kStep>(a, ++w.b);
+  while (w.rows <= 0 && w.b + 1 < a.B);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int row, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      :
+      : "r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(head), "r"(page)
+      : "memory");
+}
+
+__device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+// Query heads as operand fragments: of every 16 columns, lane l holds columns 2 (l % 4) + {0, 1, 8, 9} of head l / 4 (and of head
+// l / 4 + 8 where there are more than eight). A head's columns j and j + D / 2 are in the same lane.
+template <int D, bool kStep>
+__device__ __forceinline__ void load_head(const Args& a, const bf16* x, bool there, int pos, int lane, float (&v)[D / 16][4]) {
+  const int col = 2 * (lane & 3);
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t two = there ? *reinterpret_cast<const uint32_t*>(x + 16 * k + 8 * e + col) : 0u;
+      v[k][2 * e] = bf_lo(two);
+      v[k][2 * e + 1] = bf_hi(two);
+      ss += v[k][2 * e] * v[k][2 * e] + v[k][2 * e + 1] * v[k][2 * e + 1];
+    }
+  }
+  if constexpr (kStep) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+    ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+    if (a.st.q_w) {
+      const float r = rsqrtf(ss / D + a.st.eps);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t two = *reinterpret_cast<const uint32_t*>(static_cast<const bf16*>(a.st.q_w) + 16 * k + 8 * e + col);
+          v[k][2 * e] *= r * bf_lo(two);
+          v[k][2 * e + 1] *= r * bf_hi(two);
+        }
+      }
+    }
+    const float *cs = a.st.cos_t + static_cast<long long>(pos) * D + col, *sn = a.st.sin_t + static_cast<long long>(pos) * D + col;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = 16 * k + 8 * e;
+        const float2 c1 = *reinterpret_cast<const float2*>(cs + at), s1 = *reinterpret_cast<const float2*>(sn + at);
+        const float2 c2 = *reinterpret_cast<const float2*>(cs + at + D / 2), s2 = *reinterpret_cast<const float2*>(sn + at + D / 2);
+        float(&lo)[4] = v[k], (&hi)[4] = v[k + D / 32];
+        const float x0 = lo[2 * e], x1 = lo[2 * e + 1], y0 = hi[2 * e], y1 = hi[2 * e + 1];
+        lo[2 * e] = x0 * c1.x - y0 * s1.x;
+        lo[2 * e + 1] = x1 * c1.y - y1 * s1.y;
+        hi[2 * e] = y0 * c2.x + x0 * s2.x;
+        hi[2 * e + 1] = y1 * c2.y + x1 * s2.y;
+      }
+    }
+  }
+}
+
+// The new row's key, normalised and rotated: lane l holds columns 32 i + l.
 template <int D>
-__device__ __forceinline__ void norm_rotate(const bf16* x, const bf16* w, const float* cs, const float* sn, float eps, int lane,
-                                            float (&y)[D / 32]) {
+__device__ __forceinline__ void new_key(const Args& a, const bf16* x, int pos, int lane, bf16 (&y)[D / 32]) {
   constexpr int N = D / 32;
   float v[N], ss = 0.f;
 #pragma unroll
@@ -53,194 +180,577 @@ __device__ __forceinline__ void norm_rotate(const bf16* x, const bf16* w, const 
     v[i] = to_f32(x[lane + 32 * i]);
     ss += v[i] * v[i];
   }
-  if (w) {
-    const float r = rsqrtf(warp_sum(ss) / D + eps);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= r * to_f32(w[lane + 32 * i]);
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (a.st.k_w) {
+    const float r = rsqrtf(ss / D + a.st.eps);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= r * to_f32(static_cast<const bf16*>(a.st.k_w)[lane + 32 * i]);
   }
+  const float *cs = a.st.cos_t + static_cast<long long>(pos) * D + lane, *sn = a.st.sin_t + static_cast<long long>(pos) * D + lane;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float other = i < N / 2 ? -v[i + N / 2] : v[i - N / 2];
-    y[i] = v[i] * cs[lane + 32 * i] + other * sn[lane + 32 * i];
+    y[i] = from_f32<bf16>(v[i] * cs[32 * i] + other * sn[32 * i]);
   }
 }
 
-template <int D, int kG, bool kStep>
-__global__ void __launch_bounds__(warps_of(kG) * 32) paged_attention_kernel(Args a) {
-  constexpr int N = D / 32, kWarps = warps_of(kG);
-  __shared__ float s_q[kG][D];
-  __shared__ float s_m[kWarps][kG], s_l[kWarps][kG], s_acc[kWarps][kG][D];
+// Byte of column x of row r within a tile: halves of 64 columns, rows of 128 bytes, 16-byte pieces exchanged by the row (as TMA does).
+__device__ __forceinline__ uint32_t place(int r, int x) { return (x >> 6) * (kTile * 128) + r * 128 + ((((x >> 3) & 7) ^ (r & 7)) << 4) + (x & 7) * 2; }
+
+template <int D, bool kWide, bool kStep>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(D, kWide))
+paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
+  constexpr int kStages = stages_of(D, kWide), kHalf = kTile * D * 2;
+  constexpr int kHeads = kWide ? 2 : 1;                   // of a lane
+  constexpr int kFloats = lane_floats(D, kWide);
+  extern __shared__ unsigned char s_dyn[];
+  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ long long s_scan[kThreads / 32];
+  __shared__ Walk s_start;
+  __shared__ int s_abort;
+  unsigned char* ring = s_dyn + ((1024 - (smem_u32(s_dyn) & 1023)) & 1023);
+  float* s_merge = reinterpret_cast<float*>(ring + kStages * stage_bytes(D));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int block = blockIdx.x, blocks = gridDim.x;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_empty[s], kWarps);
+    }
+    fence_barrier_init();
+    s_abort = 0;
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
   griddep_wait();
   griddep_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y, hkv = gridDim.x, G = a.G;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int* table = a.c.table + b * a.c.table_stride;
-  const int limit = a.c.width * a.c.page;
-  int n = a.c.lengths[b];
-  const int at = n;                                     // the new row, where there is one
-  bool ok = n <= limit;
-  if constexpr (kStep) {
-    ok = n < limit;
-    if (ok && n >= 0) {
-      const int pos = a.st.positions[b], page = table[n / a.c.page];
-      ok = pos >= 0 && pos < a.st.table_rows && page >= 0 && page < a.c.pages;
+
+  // Tiles ahead of each sequence: every thread a run of sequences.
+  const int run = (a.B + kThreads - 1) / kThreads, from = min(a.B, tid * run), to = min(a.B, from + run);
+  long long mine = 0;
+  for (int b = from; b < to; ++b) {
+    const int rows = rows_of<kStep>(a, b);
+    mine += tiles_of(rows);
+    if (rows < 0 && block == 0) atomicMax(a.status, kStatusBounds);
+  }
+  long long before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += up;
+  }
+  if (lane == 31) s_scan[warp] = before;
+  before -= mine;
+  __syncthreads();
+  long long units = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_scan[w];
+    units += s_scan[w];
+  }
+  units *= a.hkv;
+  before *= a.hkv;
+  mine *= a.hkv;
+  const long long u0 = first_unit(units, block, blocks), u1 = first_unit(units, block + 1, blocks);
+  if (u1 > u0 && u0 >= before && u0 < before + mine) {
+    long long at = before;
+    int b = from, rows = 0;
+    for (;; ++b) {
+      rows = rows_of<kStep>(a, b);
+      const long long all = static_cast<long long>(tiles_of(rows)) * a.hkv;
+      if (u0 < at + all) break;
+      at += all;
     }
-    n = n < 0 ? 0 : n + 1;
+    const int tiles = tiles_of(rows), h = static_cast<int>((u0 - at) / tiles);
+    s_start = {b, h, static_cast<int>(u0 - at - static_cast<long long>(h) * tiles), rows, u1 - u0};
+    a.block_pair[block] = b * a.hkv + h;
   }
-  if (!ok) {
-    if (threadIdx.x == 0) atomicMax(a.status, kStatusBounds);
-    n = 0;
+  if (tid == 0 && block == 0) *a.units = static_cast<int>(units);
+  // sequences without rows: zeros
+  for (int b = block; b < a.B; b += blocks) {
+    if (rows_of<kStep>(a, b) > 0) continue;
+    for (int i = tid; i < a.hkv * a.G * D / 8; i += kThreads)
+      reinterpret_cast<uint4*>(a.out + static_cast<long long>(b) * a.hkv * a.G * D)[i] = make_uint4(0, 0, 0, 0);
+    for (int h = tid; h < a.hkv; h += kThreads) a.pairs[b * a.hkv + h] = {0, -1, -1, 0};
   }
-  bf16* out = a.out + (static_cast<long long>(b) * a.hq + h * G) * D;
-  if (n <= 0) {
-    for (int i = threadIdx.x; i < G * D; i += blockDim.x) out[i] = from_f32<bf16>(0.f);
+  __syncthreads();
+  if (u1 <= u0) return;
+
+  Walk w = s_start;
+  int stage = 0, phase = 0;
+  auto advance = [&] {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  };
+  if (warp == kWarps) {
+    // ------------------------------------------------------------------ feeds the ring
+    // A lane a box: the tile's page, the key or the value, the half of its columns.
+    constexpr int kParts = D / 64 * 2;
+    const int box = lane / kParts, part = lane % kParts;
+    const bool value = part >= D / 64;
+    const int x = part % (D / 64) * 64;
+    while (w.left > 0) {
+      const int tiles = tiles_of(w.rows), take = static_cast<int>(min(static_cast<long long>(tiles - w.t), w.left));
+      const int* table = a.c.table + w.b * a.c.table_stride;
+      for (int t = w.t; t < w.t + take; ++t) {
+        const int row = t * kTile + box * a.box_rows;
+        const bool mine_box = box < a.boxes && row < w.rows;
+        int page = 0;
+        if (mine_box) {
+          page = table[row / a.c.page];
+          if (page < 0 || page >= a.c.pages) {           // the map has no such page: zeros arrive
+            page = a.c.pages;
+            atomicMax(a.status, kStatusBounds);
+          }
+        }
+        if (!mbar_wait(&s_empty[stage], phase ^ 1, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
+        const int count = min(a.boxes, (w.rows - t * kTile + a.box_rows - 1) / a.box_rows);
+        if (lane == 0) mbar_arrive_expect_tx(&s_full[stage], count * kParts * a.box_rows * 128);
+        __syncwarp();
+        if (mine_box)
+          tma_load_4d(smem_u32(ring + stage * stage_bytes(D)) + (value ? kHalf : 0) + (x / 64) * (kTile * 128) + box * a.box_rows * 128,
+                      value ? &v_map : &k_map, &s_full[stage], x, row % a.c.page, w.h, page);
+        advance();
+      }
+      next_pair<kStep>(a, w, take);
+    }
     return;
   }
-  const long long pair = static_cast<long long>(b) * hkv + h;
-  const bf16* row = a.q + b * a.q_stride;
-  bf16* kp = static_cast<bf16*>(a.c.k) + h * a.c.stride_h;
-  bf16* vp = static_cast<bf16*>(a.c.v) + h * a.c.stride_h;
-  if constexpr (kStep) {
-    const int pos = a.st.positions[b];
-    const float *cs = a.st.cos_t + static_cast<long long>(pos) * D, *sn = a.st.sin_t + static_cast<long long>(pos) * D;
-    for (int g = warp; g <= G; g += kWarps) {
-      float y[N];
-      const bool key = g == G;
-      norm_rotate<D>(row + static_cast<long long>(key ? a.hq + h : h * G + g) * D, static_cast<const bf16*>(key ? a.st.k_w : a.st.q_w),
-                     cs, sn, a.st.eps, lane, y);
-      if (!key) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) s_q[g][lane + 32 * i] = y[i];
-        continue;
-      }
-      const long long to = table[at / a.c.page] * a.c.stride_p + at % a.c.page * a.c.stride_t;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        kp[to + lane + 32 * i] = from_f32<bf16>(y[i]);
-        vp[to + lane + 32 * i] = row[static_cast<long long>(a.hq + hkv + h) * D + lane + 32 * i];
-      }
-      if (lane == 0 && a.st.row_positions) a.st.row_positions[pair * limit + at] = pos;
-    }
-  } else {
-    for (int i = threadIdx.x; i < G * D; i += blockDim.x) s_q[i / D][i % D] = to_f32(row[static_cast<long long>(h) * G * D + i]);
-  }
-  __syncthreads();
 
-  float m[kG], l[kG], acc[kG][N];
+  // ---------------------------------------------------------------------- computes
+  const int g0 = lane >> 2, col = 2 * (lane & 3);
+  long long unit = u0;
+  bool handed = false;                                    // the buffers of the warps' sums are in use
+  bool first_pair = true;
+  while (w.left > 0) {
+    const int tiles = tiles_of(w.rows), take = static_cast<int>(min(static_cast<long long>(tiles - w.t), w.left));
+    const int pair = w.b * a.hkv + w.h;
+    const bool last_tile = w.t + take == tiles;
+    int pos = 0;
+    if constexpr (kStep) pos = a.st.positions[w.b];
+    const bf16* q = a.q + w.b * a.q_stride;
+    // the query heads: what bf16 holds of them and what it cuts off
+    uint32_t qh[D / 16][4], ql[kWide ? D / 16 : 1][4];
+    {
+      float v[D / 16][4];
+      load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0) * D, g0 < a.G, pos, lane, v);
 #pragma unroll
-  for (int g = 0; g < kG; ++g) {
-    m[g] = -FLT_MAX;
-    l[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[g][i] = 0.f;
-  }
-  float* scores = a.scores ? a.scores + pair * G * limit : nullptr;
-  for (int r = warp; r < n; r += kWarps) {
-    const int page = table[r / a.c.page];
-    const bool have = page >= 0 && page < a.c.pages;
-    if (!have && lane == 0) atomicMax(a.status, kStatusBounds);
-    float kf[N], vf[N];
-    const long long from = page * a.c.stride_p + r % a.c.page * a.c.stride_t;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      kf[i] = have ? to_f32(kp[from + lane + 32 * i]) : 0.f;
-      vf[i] = have ? to_f32(vp[from + lane + 32 * i]) : 0.f;
-    }
-#pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      if (g < G) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) s += s_q[g][lane + 32 * i] * kf[i];
-        s = warp_sum(s) * a.scale;
-        if (scores && lane == 0) scores[static_cast<long long>(g) * limit + r] = s;
-        if (s > m[g]) {
-          const float f = expf(m[g] - s);
-          l[g] *= f;
-#pragma unroll
-          for (int i = 0; i < N; ++i) acc[g][i] *= f;
-          m[g] = s;
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t hi[2], lo[2];
+        split_pair(v[k][0], v[k][1], hi[0], lo[0]);
+        split_pair(v[k][2], v[k][3], hi[1], lo[1]);
+        qh[k][0] = hi[0];
+        qh[k][2] = hi[1];
+        if constexpr (kWide) {
+          ql[k][0] = lo[0];
+          ql[k][2] = lo[1];
+        } else {
+          qh[k][1] = lo[0];
+          qh[k][3] = lo[1];
         }
-        const float p = expf(s - m[g]);
-        l[g] += p;
+      }
+      if constexpr (kWide) {
+        load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0 + 8) * D, g0 + 8 < a.G, pos, lane, v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[g][i] += p * vf[i];
+        for (int k = 0; k < D / 16; ++k) {
+          split_pair(v[k][0], v[k][1], qh[k][1], ql[k][1]);
+          split_pair(v[k][2], v[k][3], qh[k][3], ql[k][3]);
+        }
       }
     }
-  }
+    // the new row, by the warp whose rows include it
+    const int new_row = w.rows - 1;
+    const bool owner = kStep && last_tile && (new_row % kTile) / 16 == warp;
+    bf16 nk[D / 32], nv[D / 32];
+    if (kStep && owner) {
+      new_key<D>(a, q + static_cast<long long>(a.hkv * a.G + w.h) * D, pos, lane, nk);
+      const bf16* value = q + static_cast<long long>(a.hkv * (a.G + 1) + w.h) * D;
+      const long long at = a.c.table[w.b * a.c.table_stride + new_row / a.c.page] * a.c.stride_p + w.h * a.c.stride_h +
+                           new_row % a.c.page * a.c.stride_t;
 #pragma unroll
-  for (int g = 0; g < kG; ++g) {
-    if (lane == 0) {
-      s_m[warp][g] = m[g];
-      s_l[warp][g] = l[g];
+      for (int i = 0; i < D / 32; ++i) nv[i] = value[lane + 32 * i];
+      if (lane == 0 && a.st.row_positions)
+        a.st.row_positions[static_cast<long long>(pair) * a.c.width * a.c.page + new_row] = pos;
+      // the tile's copy is under way or has arrived: whatever it holds of this row is replaced below
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        static_cast<bf16*>(a.c.k)[at + lane + 32 * i] = nk[i];
+        static_cast<bf16*>(a.c.v)[at + lane + 32 * i] = nv[i];
+      }
+    }
+    if (w.t == 0 && tid == 0)
+      a.pairs[pair] = {static_cast<int>(unit), block, block_of(unit + tiles - 1, first_unit(units, blocks, blocks), blocks), w.rows};
+
+    float m[kHeads], l[kHeads], o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      m[i] = -FLT_MAX;
+      l[i] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) s_acc[warp][g][lane + 32 * i] = acc[g][i];
-  }
-  __syncthreads();
-  auto whole = [&](int g, float& top, float& sum) {
-    top = -FLT_MAX;
-    sum = 0.f;
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+    for (int t = w.t; t < w.t + take; ++t, ++unit) {
+      if (!mbar_wait(&s_full[stage], phase, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
+      const uint32_t ks = smem_u32(ring + stage * stage_bytes(D)), vs = ks + kHalf;
+      const int r0 = 16 * warp, valid = w.rows - t * kTile - r0;   // of this warp's 16 rows
+      if (a.unit_pair && tid == 0) a.unit_pair[unit] = pair;
+      if (valid > 0) {
+        if (kStep && owner && t == tiles - 1) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][g]);
+          for (int i = 0; i < D / 32; ++i) {
+            unsigned char* tile = ring + stage * stage_bytes(D);
+            const uint32_t at = place(new_row % kTile, lane + 32 * i);
+            *reinterpret_cast<bf16*>(tile + at) = nk[i];
+            *reinterpret_cast<bf16*>(tile + kHalf + at) = nv[i];
+          }
+          __syncwarp();
+          fence_proxy_async();                            // the next copy into this stage comes behind these writes
+        }
+        float s[2][4] = {};
+        const int key = (lane >> 4) * 8 + (lane & 7), piece = (lane >> 3) & 1;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += s_l[w][g] * expf(s_m[w][g] - top);
-  };
-  for (int i = threadIdx.x; i < G * D; i += blockDim.x) {
-    const int g = i / D, d = i - g * D;
-    float top, sum, v = 0.f;
-    whole(g, top, sum);
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t kb[4];
+          ldsm4(kb, ks + place(r0 + key, 16 * k + 8 * piece));
+          mma16816(s[0], qh[k], kb[0], kb[1]);
+          mma16816(s[1], qh[k], kb[2], kb[3]);
+          if constexpr (kWide) {
+            mma16816(s[0], ql[k], kb[0], kb[1]);
+            mma16816(s[1], ql[k], kb[2], kb[3]);
+          }
+        }
+        // p of head i of this lane at keys col + {0, 1, 8, 9}
+        uint32_t ph[4], pl[4];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += s_acc[w][g][d] * expf(s_m[w][g] - top);
-    out[i] = from_f32<bf16>(v / sum);
-  }
-  if (scores) {
-    float top[kG], inv[kG];
+        for (int i = 0; i < kHeads; ++i) {
+          float x[4];
 #pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      whole(g, top[g], inv[g]);
-      inv[g] = 1.f / inv[g];
+          for (int e = 0; e < 4; ++e) {
+            const float sum = kWide ? s[e >> 1][2 * i + (e & 1)] : s[e >> 1][e & 1] + s[e >> 1][2 + (e & 1)];
+            x[e] = col + (e & 1) + (e >> 1) * 8 < valid ? sum * a.scale_log2 : -INFINITY;
+          }
+          if (a.scores && g0 + 8 * i < a.G) {
+            float* to_scores = a.scores + (unit * a.G + g0 + 8 * i) * kTile + r0 + col;
+            *reinterpret_cast<float2*>(to_scores) = make_float2(x[0], x[1]);
+            *reinterpret_cast<float2*>(to_scores + 8) = make_float2(x[2], x[3]);
+          }
+          float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          if (top > m[i]) {                               // rare after the first tiles
+            const float f = exp2f(m[i] - top);
+            m[i] = top;
+            l[i] *= f;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              o[j][2 * i] *= f;
+              o[j][2 * i + 1] *= f;
+              if constexpr (!kWide) {
+                o[j][2] *= f;
+                o[j][3] *= f;
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = exp2f(x[e] - m[i]);
+            l[i] += x[e];
+          }
+          uint32_t hi[2], lo[2];
+          split_pair(x[0], x[1], hi[0], lo[0]);
+          split_pair(x[2], x[3], hi[1], lo[1]);
+          if constexpr (kWide) {
+            ph[i] = hi[0];
+            ph[2 + i] = hi[1];
+            pl[i] = lo[0];
+            pl[2 + i] = lo[1];
+          } else {
+            ph[0] = hi[0];
+            ph[1] = lo[0];
+            ph[2] = hi[1];
+            ph[3] = lo[1];
+          }
+        }
+        // values behind the end may be anything: 0 times NaN is not 0
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (valid < 16) {
+          keep0 = (col < valid ? 0x0000ffffu : 0u) | (col + 1 < valid ? 0xffff0000u : 0u);
+          keep1 = (col + 8 < valid ? 0x0000ffffu : 0u) | (col + 9 < valid ? 0xffff0000u : 0u);
+        }
+        const int vkey = ((lane >> 3) & 1) * 8 + (lane & 7), vpiece = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          uint32_t vb[4];
+          ldsm4_t(vb, vs + place(r0 + vkey, 16 * j + 8 * vpiece));
+          if (valid < 16) {
+            vb[0] &= keep0;
+            vb[1] &= keep1;
+            vb[2] &= keep0;
+            vb[3] &= keep1;
+          }
+          mma16816(o[2 * j], ph, vb[0], vb[1]);
+          mma16816(o[2 * j + 1], ph, vb[2], vb[3]);
+          if constexpr (kWide) {
+            mma16816(o[2 * j], pl, vb[0], vb[1]);
+            mma16816(o[2 * j + 1], pl, vb[2], vb[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[stage]);
+      advance();
     }
-    float* weights = a.c.weights + pair * limit;
-    for (int r = threadIdx.x; r < n; r += blockDim.x) {
-      float share = kStep && r == at ? 0.f : weights[r];
-      for (int g = 0; g < G; ++g) share += expf(scores[static_cast<long long>(g) * limit + r] - top[g]) * inv[g];
-      weights[r] = share;
+
+    // The four warps' sums meet in the first, lane by lane (all hold the same heads and columns).
+    float f[kFloats];
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      if constexpr (kWide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * j + e] = o[j][e];
+      } else {
+        f[2 * j] = o[j][0] + o[j][2];
+        f[2 * j + 1] = o[j][1] + o[j][3];
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    if (handed) warps_sync();                             // the first warp has read the last pair's
+    handed = true;
+    if (warp > 0) {
+      float* to_first = s_merge + (warp - 1) * 32 * (kFloats + 4);
+#pragma unroll
+      for (int x = 0; x < kFloats / 4; ++x)
+        reinterpret_cast<float4*>(to_first)[x * 32 + lane] = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
+      reinterpret_cast<float4*>(to_first)[kFloats / 4 * 32 + lane] = make_float4(m[0], l[0], m[kHeads - 1], l[kHeads - 1]);
+    }
+    warps_sync();
+    if (warp == 0) {
+#pragma unroll
+      for (int other = 0; other < kWarps - 1; ++other) {
+        const float4* s = reinterpret_cast<const float4*>(s_merge + other * 32 * (kFloats + 4));
+        const float4 ml = s[kFloats / 4 * 32 + lane];
+        float own[kHeads], its[kHeads];
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          const float om = i ? ml.z : ml.x, ol = i ? ml.w : ml.y, top = fmaxf(m[i], om);
+          own[i] = exp2f(m[i] - top);
+          its[i] = exp2f(om - top);
+          l[i] = l[i] * own[i] + ol * its[i];
+          m[i] = top;
+        }
+#pragma unroll
+        for (int x = 0; x < kFloats / 4; ++x) {
+          const float4 v = s[x * 32 + lane];
+          // pairs of columns: of one head, or of the lane's two in turn
+          f[4 * x] = f[4 * x] * own[0] + v.x * its[0];
+          f[4 * x + 1] = f[4 * x + 1] * own[0] + v.y * its[0];
+          f[4 * x + 2] = f[4 * x + 2] * own[kHeads - 1] + v.z * its[kHeads - 1];
+          f[4 * x + 3] = f[4 * x + 3] * own[kHeads - 1] + v.w * its[kHeads - 1];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const int g = g0 + 8 * i;
+        if (g < a.G) {
+          if (w.t == 0 && last_tile) {                    // the whole pair
+            const float inv = 1.f / l[i];
+            bf16* out = a.out + (static_cast<long long>(pair) * a.G + g) * D + col;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j)
+              *reinterpret_cast<uint32_t*>(out + 8 * j) =
+                  bf_pack(f[2 * kHeads * j + 2 * i] * inv, f[2 * kHeads * j + 2 * i + 1] * inv);
+            if (a.top_sum && (lane & 3) == 0) a.top_sum[pair * a.G + g] = make_float2(m[i], l[i]);
+          } else {
+            float* part = a.part + (2LL * block + (first_pair ? 0 : 1)) * a.G * (D + 2);
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j)
+              *reinterpret_cast<float2*>(part + g * D + 8 * j + col) =
+                  make_float2(f[2 * kHeads * j + 2 * i], f[2 * kHeads * j + 2 * i + 1]);
+            if ((lane & 3) == 0) {
+              part[a.G * D + 2 * g] = m[i];
+              part[a.G * D + 2 * g + 1] = l[i];
+            }
+          }
+        }
+      }
+    }
+    first_pair = false;
+    next_pair<kStep>(a, w, take);
   }
 }
 
+// The sums of block `c`'s part of a pair.
+__device__ __forceinline__ const float* part_of(const Args& a, const Pair& p, int c, long long units, int blocks, int D) {
+  const bool starts = first_unit(units, c, blocks) >= p.unit;     // the block begins with this pair
+  return a.part + (2LL * c + (starts ? 0 : 1)) * a.G * (D + 2);
+}
+
+constexpr int kFinishThreads = 256;
+
+// Pairs that several blocks share: block c those whose first cut is the start of stretch c. Then the weights, a warp a tile.
 template <bool kStep>
-cudaError_t launch_any(const Args& a, int B, int hkv, int D, cudaStream_t stream) {
-  const dim3 grid(hkv, B);
-#define CDEEP_PAGED(DD, GG) \
-  if (D == DD && a.G <= GG) return launch_kernel(paged_attention_kernel<DD, GG, kStep>, grid, dim3(warps_of(GG) * 32), 0, stream, a);
-  CDEEP_PAGED(64, 2) CDEEP_PAGED(64, 4) CDEEP_PAGED(64, 8) CDEEP_PAGED(64, 16)
-  CDEEP_PAGED(128, 2) CDEEP_PAGED(128, 4) CDEEP_PAGED(128, 8) CDEEP_PAGED(128, 16)
-#undef CDEEP_PAGED
-  return cudaErrorInvalidValue;
+__global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args a, int blocks, int D) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long units = *a.units;
+  const int tid = threadIdx.x, G = a.G;
+  if (units == 0) return;
+  if (blockIdx.x > 0 && static_cast<int>(blockIdx.x) < blocks) {
+    const int c = blockIdx.x;
+    const long long u = first_unit(units, c, blocks);
+    if (u < first_unit(units, c + 1, blocks)) {
+      const int pair = a.block_pair[c];
+      const Pair p = a.pairs[pair];
+      // the stretches ahead that are empty begin at the same tile
+      if (p.unit < u && p.first < c && block_of(u - 1, units, blocks) == p.first) {
+        for (int i = tid; i < G * D; i += kFinishThreads) {
+          const int g = i / D;
+          float m = -FLT_MAX, l = 0.f, v = 0.f;
+          for (int x = p.first; x <= p.last; ++x) {
+            if (first_unit(units, x, blocks) == first_unit(units, x + 1, blocks)) continue;
+            const float* part = part_of(a, p, x, units, blocks, D);
+            const float pm = part[G * D + 2 * g], top = fmaxf(m, pm), f = exp2f(m - top), e = exp2f(pm - top);
+            v = v * f + part[i] * e;
+            l = l * f + part[G * D + 2 * g + 1] * e;
+            m = top;
+          }
+          a.out[static_cast<long long>(pair) * G * D + i] = from_f32<bf16>(v / l);
+        }
+      }
+    }
+  }
+  if (!a.scores) return;
+  const int lane = tid & 31;
+  const long long limit = static_cast<long long>(a.c.width) * a.c.page;
+  for (long long u = blockIdx.x * (kFinishThreads / 32LL) + (tid >> 5); u < units; u += gridDim.x * (kFinishThreads / 32LL)) {
+    const int pair = a.unit_pair[u];
+    const Pair p = a.pairs[pair];
+    float top = 0.f, inv = 0.f;                           // lane g: of head g
+    if (lane < G) {
+      float m = -FLT_MAX, l = 0.f;
+      if (p.first == p.last) {
+        const float2 ml = a.top_sum[pair * G + lane];
+        m = ml.x;
+        l = ml.y;
+      } else {
+        for (int x = p.first; x <= p.last; ++x) {
+          if (first_unit(units, x, blocks) == first_unit(units, x + 1, blocks)) continue;
+          const float* part = part_of(a, p, x, units, blocks, D) + G * D + 2 * lane;
+          const float next = fmaxf(m, part[0]);
+          l = l * exp2f(m - next) + part[1] * exp2f(part[0] - next);
+          m = next;
+        }
+      }
+      top = m;
+      inv = 1.f / l;
+    }
+    const int row = static_cast<int>(u - p.unit) * kTile + 2 * lane;
+    float s0 = 0.f, s1 = 0.f;
+    for (int g = 0; g < G; ++g) {
+      const float2 s = *reinterpret_cast<const float2*>(a.scores + (u * G + g) * kTile + 2 * lane);
+      const float tg = __shfl_sync(0xffffffffu, top, g), ig = __shfl_sync(0xffffffffu, inv, g);
+      s0 += exp2f(s.x - tg) * ig;
+      s1 += exp2f(s.y - tg) * ig;
+    }
+    float* w = a.c.weights + pair * limit + row;
+    if (row < p.rows) w[0] = (kStep && row == p.rows - 1 ? 0.f : w[0]) + s0;
+    if (row + 1 < p.rows) w[1] = (kStep && row + 1 == p.rows - 1 ? 0.f : w[1]) + s1;
+  }
+}
+
+int sm_count() {
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 148;
+  return n;
+}
+
+// Where things lie in the workspace; blocks is what the launch has at most, whatever the device.
+struct Layout {
+  long long tiles;
+  size_t block_pair, pairs, part, unit_pair, top_sum, scores, bytes;
+};
+constexpr int kMostBlocks = 2 * 160;
+Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
+  Layout l = {};
+  auto take = [&](size_t n) {
+    const size_t at = l.bytes;
+    l.bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  const long long rows = static_cast<long long>(width) * page, pairs = static_cast<long long>(B) * hkv;
+  l.tiles = pairs * ((rows + kTile - 1) / kTile);
+  l.bytes = 256;                                          // units
+  l.block_pair = take(sizeof(int) * kMostBlocks);
+  l.pairs = take(sizeof(Pair) * pairs);
+  l.part = take(sizeof(float) * kMostBlocks * 2 * G * (D + 2));
+  l.unit_pair = weights ? take(sizeof(int) * l.tiles) : 0;
+  l.top_sum = weights ? take(sizeof(float2) * pairs * G) : 0;
+  l.scores = weights ? take(sizeof(float) * l.tiles * G * kTile) : 0;
+  return l;
+}
+
+template <int D, bool kWide, bool kStep>
+cudaError_t launch_one(const CUtensorMap& k, const CUtensorMap& v, const Args& a, long long tiles, cudaStream_t stream) {
+  constexpr auto kKernel = paged_attention_kernel<D, kWide, kStep>;
+  cudaError_t e = allow_smem<kKernel>(smem_bytes(D, kWide));
+  if (e != cudaSuccess) return e;
+  const long long most = sm_count() * blocks_per_sm(D, kWide) < kMostBlocks ? sm_count() * blocks_per_sm(D, kWide) : kMostBlocks;
+  const int blocks = static_cast<int>(tiles < most ? tiles : most);
+  e = launch_kernel(kKernel, dim3(blocks), dim3(kThreads), smem_bytes(D, kWide), stream, k, v, a);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(paged_finish_kernel<kStep>, dim3(a.scores && blocks > 8 ? 2 * blocks : blocks), dim3(kFinishThreads), 0, stream, a, blocks, D);
 }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int B, int hq, int, int, int page, int width, bool weights) {
-  return weights ? sizeof(float) * B * hq * width * page : 0;
+size_t paged_attention_workspace_bytes(int B, int hq, int hkv, int D, int page, int width, bool weights) {
+  return layout(B, hkv, hq / hkv, D, page, width, weights).bytes;
 }
 
 cudaError_t launch_paged_attention(const cd_paged& c, const cd_paged_step* step, const void* q, long long q_stride, float scale, int B,
                                    int hq, int hkv, int D, void* out, void* ws, int* status, cudaStream_t stream) {
+  const Layout l = layout(B, hkv, hq / hkv, D, c.page, c.width, c.weights != nullptr);
+  char* base = static_cast<char*>(ws);
   Args a;
   a.c = c;
   a.q = static_cast<const bf16*>(q);
   a.q_stride = q_stride;
   a.st = step ? *step : cd_paged_step{};
-  a.scale = scale;
+  a.scale_log2 = scale * kLog2e;
+  a.B = B;
+  a.hkv = hkv;
   a.G = hq / hkv;
-  a.hq = hq;
+  a.box_rows = c.page < kTile ? c.page : kTile;
+  a.boxes = kTile / a.box_rows;
   a.out = static_cast<bf16*>(out);
-  a.scores = c.weights ? static_cast<float*>(ws) : nullptr;
   a.status = status;
-  return step ? launch_any<true>(a, B, hkv, D, stream) : launch_any<false>(a, B, hkv, D, stream);
+  a.units = reinterpret_cast<int*>(base);
+  a.block_pair = reinterpret_cast<int*>(base + l.block_pair);
+  a.pairs = reinterpret_cast<Pair*>(base + l.pairs);
+  a.part = reinterpret_cast<float*>(base + l.part);
+  a.unit_pair = c.weights ? reinterpret_cast<int*>(base + l.unit_pair) : nullptr;
+  a.top_sum = c.weights ? reinterpret_cast<float2*>(base + l.top_sum) : nullptr;
+  a.scores = c.weights ? reinterpret_cast<float*>(base + l.scores) : nullptr;
+  CUtensorMap k, v;
+  const int dims[4] = {D, c.page, hkv, c.pages};
+  const long long strides[3] = {c.stride_t, c.stride_h, c.stride_p};
+  if (!encode_map_4d(&k, c.k, dims, strides, a.box_rows) || !encode_map_4d(&v, c.v, dims, strides, a.box_rows))
+    return cudaErrorInvalidValue;
+#define CDEEP_PAGED(DD, WIDE)                                                                                     \
+  if (D == DD && (a.G > 8) == WIDE)                                                                               \
+    return step ? launch_one<DD, WIDE, true>(k, v, a, l.tiles, stream) : launch_one<DD, WIDE, false>(k, v, a, l.tiles, stream);
+  CDEEP_PAGED(64, false) CDEEP_PAGED(64, true) CDEEP_PAGED(128, false) CDEEP_PAGED(128, true)
+#undef CDEEP_PAGED
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace cdeep

@@ -1496,6 +1496,10 @@ def paged_step_attention(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Op
     if cos.dim() != 2:
         raise RuntimeError("cos/sin: expected [positions, head_dim]")
     table = (cos.shape[0], D)
+    if (cos.data_ptr() | sin.data_ptr()) & 7:
+        cos, sin = cos.clone(), sin.clone()
+    if q_w is not None and q_w.data_ptr() & 3:
+        q_w = q_w.clone()
     step = _lib.PagedStep(
         None if q_w is None else _on(q_w, "q_norm.weight", BF16, device, (D,)),
         None if k_w is None else _on(k_w, "k_norm.weight", BF16, device, (D,)),

@@ -684,9 +684,9 @@ typedef struct cd_paged {
 
 /* What a decode step brings besides the projections. */
 typedef struct cd_paged_step {
-  const void* q_w;          /* [D] norm weights, or both NULL */
+  const void* q_w;          /* [D] norm weights (q_w on a 4-byte boundary), or both NULL */
   const void* k_w;
-  const float* cos_t;       /* [table_rows, D] */
+  const float* cos_t;       /* [table_rows, D], on 8-byte boundaries */
   const float* sin_t;
   const int32_t* positions; /* [B] of the new tokens */
   int32_t* row_positions;   /* [B, kv heads, width * page] position of every cached row, or NULL */
