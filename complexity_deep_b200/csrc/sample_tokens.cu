@@ -4,8 +4,9 @@
 //   index, i stays where the mass ahead of it is at most p times the mass that top-k has left;  min-p: w_i >= min_p;
 //   id = the first i, in the order of the vocabulary, with sum_{j <= i} w_j > u sum_j w_j over what stayed.
 //
-// The result is a whole number that hangs on where sums lie next to a border, so weights are 64-bit exponentials, held as multiples
-// of 2^-44: sums of up to 2^18 of them are exact, and the same in any order.
+// The result is a whole number that hangs on where sums lie next to a border, so weights are good to 2^-32 of themselves and held as
+// multiples of 2^-44: sums of up to 2^18 of them are exact, and the same in any order. Nine products and sums in 32 bits and one of
+// whole numbers give such a weight (Row::mass); in 64-bit arithmetic it took 2.6 times as long (64 rows of 100 000: 94 us).
 //
 // A cluster of blocks a row, which is read once and stays in their shared memory. A warp has a stretch of neighbouring tokens, its
 // lanes take 16 bytes of it in turn.
@@ -27,22 +28,43 @@ namespace cdeep {
 
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
-constexpr int kBins = 2048;
 constexpr int kList = 512;                 // entries compared pair by pair
-constexpr int kFew = 256;                  // the largest k that takes the bound
+constexpr int kFew = 192;                  // the largest k that takes the bound
 constexpr int kMostBlocks = 8;             // of a row: the largest cluster that every device takes
-constexpr int kSliceBytes = 128 * 1024;    // of a row that a block holds at most: 2^18 numbers of 32 bits are eight
+constexpr int kSliceBytes = 144 * 1024;    // of a row in a block: 2^18 numbers of 32 bits are eight blocks of 128 KB
 using u64 = unsigned long long;
 constexpr u64 kOne = 1ull << 44;
 
-// Order of logits as unsigned numbers; NaN below -inf.
-__device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return x != x ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-constexpr uint32_t kMinusInf = 0x007fffffu;
+// Order of logits as unsigned numbers, NaN below -inf; bf16 in the upper half.
+template <typename T>
+struct Key;
+template <>
+struct Key<float> {
+  static constexpr uint32_t kMinusInf = 0x007fffffu;
+  static __device__ __forceinline__ uint32_t of(uint32_t bits) {
+    const uint32_t u = __float_as_uint(__uint_as_float(bits) + 0.f);         // -0 is 0
+    const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
+    return (bits & 0x7fffffffu) > 0x7f800000u ? 0u : k;
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    return __uint_as_float(k ^ (~static_cast<uint32_t>(static_cast<int>(k) >> 31) | 0x80000000u));
+  }
+  // keys of 16 bytes of logits, and back
+  static __device__ __forceinline__ uint4 pack(const uint32_t (&k)[4]) { return make_uint4(k[0], k[1], k[2], k[3]); }
+  static __device__ __forceinline__ uint32_t unpack(const uint32_t (&w)[4], int e) { return w[e]; }
+};
+template <>
+struct Key<bf16> {
+  static constexpr uint32_t kMinusInf = 0x007f0000u;
+  static __device__ __forceinline__ uint32_t of(uint32_t bits) { return Key<float>::of(bits) & 0xffff0000u; }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    return __uint_as_float((k ^ (~static_cast<uint32_t>(static_cast<int>(k) >> 31) | 0x80000000u)) & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint4 pack(const uint32_t (&k)[8]) {
+    return make_uint4(k[0] >> 16 | k[1], k[2] >> 16 | k[3], k[4] >> 16 | k[5], k[6] >> 16 | k[7]);
+  }
+  static __device__ __forceinline__ uint32_t unpack(const uint32_t (&w)[4], int e) { return e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16; }
+};
 // One order of all tokens: by value, ties by the lowest index.
 __device__ __forceinline__ u64 token(uint32_t key, int i) { return static_cast<u64>(key) << 32 | ~static_cast<uint32_t>(i); }
 
@@ -61,28 +83,32 @@ __device__ __forceinline__ u64 peer64(const void* p, int rank) {
   return v;
 }
 
+template <int kThreads>
 struct Shared {
-  double powers[64];                       // 2^(j / 64 + 44)
+  static constexpr int kWarps = kThreads / 32, kBins = 2 * kThreads;
+  u64 list[kList + 4], mass[kList + 4];    // tokens; their masses
+  u64 sorted[kList];
+  unsigned all_tops[kThreads + 4];
+  unsigned powers[256];                    // 2^(j / 256 + 31)
   u64 sums[kWarps];
   u64 total;                               // of this block, for the others
-  u64 list[kList];                         // tokens; of this block, then (in the first) of all
-  u64 mass[kList], sorted[kList];
   u64 found, before;
   unsigned hist[3][kBins];
-  unsigned tops[kThreads], all_tops[kThreads];
+  unsigned tops[kThreads];
   unsigned high, low, tau, count, key;
+  unsigned counts[kMostBlocks];
   int bin;
 };
 
-template <typename T>
+template <typename T, int kThreads>
 struct Row {
   static constexpr int kVec = 16 / sizeof(T);
-  Shared* s;
+  Shared<kThreads>* s;
   const uint4* data;                       // this block's share of the row
   int begin, stretch;                      // its first token, tokens of a warp
   int rank, blocks;
   uint32_t best;
-  double top, rate;                        // rate: 64 log2 e / T
+  float top, rate, rate_low;               // 256 log2 e / T as two numbers
 
   __device__ __forceinline__ void sync() const {
     if (blocks > 1) {
@@ -91,7 +117,7 @@ struct Row {
       __syncthreads();
     }
   }
-  // f(key, token index) for this thread's share; -inf and NaN are left out
+  // f(key, token index) for this thread's share; -inf and NaN are the keys up to kMinusInf
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     const int lane = threadIdx.x & 31, from = (threadIdx.x >> 5) * stretch;
@@ -102,26 +128,29 @@ struct Row {
     const uint4 q = data[v / kVec];
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const float x = sizeof(T) == 4 ? __uint_as_float(w[e * sizeof(T) / 4]) : e & 1 ? bf_hi(w[e / 2 % 4]) : bf_lo(w[e / 2 % 4]);
-      const uint32_t k = key_of(x);
-      if (k > kMinusInf) f(k, begin + v + e);
-    }
+    for (int e = 0; e < kVec; ++e) f(Key<T>::unpack(w, e), begin + v + e);
   }
-  // exp((x - max) / T) as a multiple of 2^-44: 2^(n / 64) from the table, the rest by a Taylor polynomial (error 2^-44)
+  // exp((x - max) / T) as a multiple of 2^-44, good to 2^-32 of itself: y = (x - max) 256 log2 e / T as a sum of two numbers, the
+  // whole part n of its 256ths from the table, 2^(f / 256) = 1 + q of the rest by a polynomial, q in 2^-31ths.
   __device__ __forceinline__ u64 mass(uint32_t key) const {
-    if (key == best) return kOne;
-    const double y = (static_cast<double>(value_of(key)) - top) * rate;
-    if (!(y > -64.0 * 46)) return 0;
-    const double t = y + 6755399441055744.0;              // 1.5 2^52: rounds to a whole number, in the low bits
-    const int n = __double2loint(t);
-    const double r = (y - (t - 6755399441055744.0)) * 0.010830424696249145;   // ln 2 / 64
-    double p = fma(r, 1.0 / 24, 1.0 / 6);
-    p = fma(r, p, 0.5);
-    p = fma(r, p, 1.0);
-    p = fma(r, p, 1.0) * s->powers[n & 63];
-    p = __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p));
-    return __double_as_longlong(p + 4503599627370496.0) & 0xfffffffffffffull;   // + 2^52: rounds, the number in the low bits
+    const float x = Key<T>::value(key), d = x - top;
+    float rest = 0.f;
+    if constexpr (sizeof(T) == 4) {                       // what the difference has lost (of bf16 numbers: nothing that counts)
+      const float back = d - x;
+      rest = (x - (d - back)) - (top + back);
+    }
+    const float y = d * rate;
+    const float low = fmaf(d, rate_low, fmaf(rest, rate, fmaf(d, rate, -y)));
+    const float t = y + 12582912.f;                       // 1.5 2^23: rounds to a whole number, in the low bits
+    const int n = __float_as_int(t) - 0x4b400000;
+    const float f = (y - (t - 12582912.f)) + low;
+    const float q = f * fmaf(f, fmaf(f, 3.3083e-9f, 3.66556e-6f), 2.7076062e-3f);       // (ln 2 / 256)^i / i!
+    const int q31 = __float_as_int(q + 5.859375e-3f) - 0x3bc00000;                      // 1.5 2^-8
+    const u64 w = static_cast<u64>(s->powers[n & 255]) * (0x80000000u + q31);           // times 2^62
+    const int shift = (18 - (n >> 8)) & 63;
+    const u64 m = (w + (1ull << (shift - 1))) >> shift;
+    // at the largest exactly 1, also where that is infinite; below 2^-45, and at -inf, 0
+    return key == best ? kOne : y > -256.f * 45 ? m : 0;
   }
 };
 
@@ -149,13 +178,23 @@ __device__ __forceinline__ u64 block_before(u64 v, u64* sums) {
   const u64 ahead = warp_sum(lane < warp ? sums[lane] : 0);
   return ahead + upto - v;
 }
-__device__ __forceinline__ u64 all_sums(const u64* sums) { return warp_sum(sums[threadIdx.x & 31]); }
+template <int kWarps>
+__device__ __forceinline__ u64 all_sums(const u64 (&sums)[kWarps]) { return warp_sum((threadIdx.x & 31) < kWarps ? sums[threadIdx.x & 31] : 0); }
+
+// f(j) for the pairs of entries of a list of n, which goes on for four more that do not count.
+template <typename F>
+__device__ __forceinline__ void pairs(int n, F f) {
+  for (int j = 0; j < n; j += 4) {
+    f(j);
+    f(j + 2);
+  }
+}
 
 // Lists the tokens that `takes` holds for, in every block those of all blocks. Returns how many there are; more than kList are not
 // kept.
-template <typename T, typename F>
-__device__ __forceinline__ unsigned collect(const Row<T>& r, F takes) {
-  Shared& s = *r.s;
+template <typename T, int kThreads, typename F>
+__device__ __forceinline__ unsigned collect(const Row<T, kThreads>& r, F takes) {
+  Shared<kThreads>& s = *r.s;
   __syncthreads();
   if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
@@ -167,14 +206,16 @@ __device__ __forceinline__ unsigned collect(const Row<T>& r, F takes) {
   });
   r.sync();
   if (r.blocks == 1) return s.count;
+  if (threadIdx.x < r.blocks) s.counts[threadIdx.x] = peer32(&s.count, threadIdx.x);
+  __syncthreads();
   unsigned all = 0;
-  for (int b = 0; b < r.blocks; ++b) all += peer32(&s.count, b);
+  for (int b = 0; b < r.blocks; ++b) all += s.counts[b];
   if (all <= kList) {                      // every block has them all, in the same places
     u64 t = 0;
     if (threadIdx.x < all) {
       unsigned at = threadIdx.x;
       int b = 0;
-      for (unsigned m; at >= (m = peer32(&s.count, b)); ++b) at -= m;
+      for (; at >= s.counts[b]; ++b) at -= s.counts[b];
       t = peer64(&s.list[at], b);
     }
     r.sync();
@@ -185,9 +226,9 @@ __device__ __forceinline__ unsigned collect(const Row<T>& r, F takes) {
 }
 
 // Sum over all blocks; s.before: that of the blocks ahead of this one, s.sums: those of its warps.
-template <typename T>
-__device__ __forceinline__ u64 row_sum(const Row<T>& r, u64 own) {
-  Shared& s = *r.s;
+template <typename T, int kThreads>
+__device__ __forceinline__ u64 row_sum(const Row<T, kThreads>& r, u64 own) {
+  Shared<kThreads>& s = *r.s;
   __syncthreads();
   const u64 w = warp_sum(own);
   if ((threadIdx.x & 31) == 0) s.sums[threadIdx.x >> 5] = w;
@@ -213,9 +254,10 @@ __device__ __forceinline__ u64 row_sum(const Row<T>& r, u64 own) {
 }
 
 // The r-th (from 0) of the tokens with this key, in the order of the vocabulary; all if there are no more than r.
-template <typename T>
-__device__ __forceinline__ int nth_equal(const Row<T>& r, uint32_t key, u64 nth) {
-  Shared& s = *r.s;
+template <typename T, int kThreads>
+__device__ __forceinline__ int nth_equal(const Row<T, kThreads>& r, uint32_t key, u64 nth) {
+  constexpr int kVec = Row<T, kThreads>::kVec;
+  Shared<kThreads>& s = *r.s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) s.found = ~0ull;
   u64 own = 0;
@@ -224,8 +266,8 @@ __device__ __forceinline__ int nth_equal(const Row<T>& r, uint32_t key, u64 nth)
   const u64 mine = s.sums[warp];
   u64 before = s.before + warp_sum(lane < warp ? s.sums[lane] : 0);
   if (before <= nth && nth < before + mine) {             // it lies in this warp's stretch
-    for (int v0 = warp * r.stretch; v0 < (warp + 1) * r.stretch; v0 += 32 * Row<T>::kVec) {
-      const int v = v0 + lane * Row<T>::kVec;
+    for (int v0 = warp * r.stretch; v0 < (warp + 1) * r.stretch; v0 += 32 * kVec) {
+      const int v = v0 + lane * kVec;
       u64 n = 0;
       if (v < (warp + 1) * r.stretch) r.vec(v, [&](uint32_t k, int) { n += k == key; });
       const u64 upto = warp_upto(n);
@@ -246,42 +288,46 @@ __device__ __forceinline__ int nth_equal(const Row<T>& r, uint32_t key, u64 nth)
 
 // The last token, in descending order through the keys from `high` down to `low` (both there), that has at most so much ahead of it:
 // `left` tokens, or (kMass) that fraction of the mass of all. For counts only the key of the result means something.
-template <bool kMass, typename T>
-__device__ __forceinline__ u64 border(const Row<T>& r, uint32_t low, uint32_t high, u64 left) {
-  Shared& s = *r.s;
+template <bool kMass, typename T, int kThreads>
+__device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, uint32_t high, u64 left) {
+  constexpr int kBins = Shared<kThreads>::kBins;
+  Shared<kThreads>& s = *r.s;
   const int tid = threadIdx.x;
   bool first = true;
   while (low < high) {
     // equal steps of the value behind the largest, which has bin 0 to itself: every turn leaves it behind or ends with it
-    const float most = value_of(high);
-    const float steps = static_cast<float>((kBins - 1) / (static_cast<double>(most) - static_cast<double>(value_of(low))));
-    auto bin_of = [&](uint32_t k) { return k == high ? 0 : 1 + min(kBins - 2, __float2int_rz((most - value_of(k)) * steps)); };
+    const float most = Key<T>::value(high);
+    const float steps = static_cast<float>((kBins - 2) / (static_cast<double>(most) - static_cast<double>(Key<T>::value(low))));
+    // 2^23 + 1 and up: rounded to whole numbers, in the low bits (fminf takes the number where the other is NaN)
+    auto bin_of = [&](uint32_t k) {
+      const float at = fminf((most - Key<T>::value(k)) * steps, kBins - 2.f) + 8388609.f;
+      return k == high ? 0 : __float_as_int(at) & (kBins - 1);
+    };
     for (int i = tid; i < (kMass ? 3 : 1) * kBins; i += kThreads) (&s.hist[0][0])[i] = 0;
     if (tid == 0) s.bin = -1, s.high = 0, s.low = 0xffffffffu;
     __syncthreads();
     r.each([&](uint32_t k, int) {
-      if (k < low || k > high) return;
       const int b = bin_of(k);
+      const u64 m = kMass ? r.mass(k) : 1;
+      if (k < low || k > high) return;
       if constexpr (kMass) {
-        const u64 m = r.mass(k);
-        const unsigned m0 = m & 0x7fff, m1 = m >> 15 & 0x7fff, m2 = static_cast<unsigned>(m >> 30);
-        if (m0) atomicAdd(&s.hist[0][b], m0);
-        if (m1) atomicAdd(&s.hist[1][b], m1);
-        if (m2) atomicAdd(&s.hist[2][b], m2);
+        atomicAdd(&s.hist[0][b], static_cast<unsigned>(m & 0x7fff));
+        atomicAdd(&s.hist[1][b], static_cast<unsigned>(m >> 15 & 0x7fff));
+        atomicAdd(&s.hist[2][b], static_cast<unsigned>(m >> 30));
       } else {
         atomicAdd(&s.hist[0][b], 1u);
       }
     });
     r.sync();
-    u64 held[2];
+    u64 held[2] = {0, 0};
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      held[x] = 0;
-      for (int b = 0; b < r.blocks; ++b) {
+    for (int b = 0; b < kMostBlocks; ++b) {
+      if (b < r.blocks) {
 #pragma unroll
         for (int e = 0; e < (kMass ? 3 : 1); ++e) {
-          const unsigned* at = &s.hist[e][2 * tid + x];
-          held[x] += static_cast<u64>(r.blocks > 1 ? peer32(at, b) : *at) << 15 * e;
+          const u64 two = peer64(&s.hist[e][2 * tid], b);
+          held[0] += (two & 0xffffffffu) << 15 * e;
+          held[1] += two >> 32 << 15 * e;
         }
       }
     }
@@ -297,7 +343,7 @@ __device__ __forceinline__ u64 border(const Row<T>& r, uint32_t low, uint32_t hi
     left -= s.before;
     unsigned hi = 0, lo = 0xffffffffu;
     const unsigned n = collect(r, [&](uint32_t k, int) {
-      if (k < low || k > high || bin_of(k) != bin) return false;
+      if (bin_of(k) != bin || k < low || k > high) return false;
       hi = max(hi, k);
       lo = min(lo, k);
       return true;
@@ -305,12 +351,20 @@ __device__ __forceinline__ u64 border(const Row<T>& r, uint32_t low, uint32_t hi
     if (n <= kList) {
       const u64 mine = tid < n ? s.list[tid] : 0;
       if (tid < n && kMass) s.mass[tid] = r.mass(static_cast<uint32_t>(mine >> 32));
+      if (tid < 4) s.list[n + tid] = 0;                     // behind everything
       if (tid == 0) s.found = ~0ull;
       __syncthreads();
       if (tid < n) {
         u64 ahead = 0;
-        for (int j = 0; j < n; ++j)
-          if (s.list[j] > mine) ahead += kMass ? s.mass[j] : 1;
+        pairs(n, [&](int j) {
+          const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(&s.list[j]);
+          if constexpr (kMass) {
+            const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(&s.mass[j]);
+            ahead += (t.x > mine ? m.x : 0) + (t.y > mine ? m.y : 0);
+          } else {
+            ahead += (t.x > mine) + (t.y > mine);
+          }
+        });
         if (ahead <= left) atomicMin(&s.found, mine);
       }
       __syncthreads();
@@ -344,20 +398,20 @@ __device__ __forceinline__ u64 border(const Row<T>& r, uint32_t low, uint32_t hi
   return token(high, nth_equal(r, high, m > 0 ? left / m : ~0ull));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits, long long ld, int V, int slice, int stretch, cd_sample p,
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kernel(const T* logits, long long ld, int V, int slice, int stretch, cd_sample p,
                                                                  long long* ids, float* probs) {
-  constexpr int kVec = Row<T>::kVec;
+  constexpr int kVec = Row<T, kThreads>::kVec, kWarps = kThreads / 32;
   extern __shared__ uint4 s_dyn[];
-  Shared& s = *reinterpret_cast<Shared*>(s_dyn);
-  uint4* s_data = s_dyn + (sizeof(Shared) + 15) / 16;
+  Shared<kThreads>& s = *reinterpret_cast<Shared<kThreads>*>(s_dyn);
+  uint4* s_data = s_dyn + (sizeof(s) + 15) / 16;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < 64) s.powers[tid] = exp2(tid / 64.0 + 44.0);
-  if (tid == 0) s.key = 0, s.low = 0xffffffffu, s.tau = 0;
+  if (tid < 256) s.powers[tid] = static_cast<unsigned>(exp2(tid / 256.0 + 31.0) + 0.5);
+  if (tid == 0) s.key = 0, s.low = 0xffffffffu, s.tau = 0, s.count = 0;
   __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
-  Row<T> r;
+  Row<T, kThreads> r;
   r.s = &s;
   r.data = s_data;
   r.blocks = gridDim.x;
@@ -374,23 +428,41 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits
   // the row's share into shared memory, NaN behind its end
   uint32_t high = 0, low = 0xffffffffu;
   const bool whole = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  for (int v = warp * stretch + lane * kVec; v < (warp + 1) * stretch; v += 32 * kVec) {
-    uint4 q = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
-    if (whole && v + kVec <= length) {
-      q = *reinterpret_cast<const uint4*>(x + v);
-    } else {
-      T* e = reinterpret_cast<T*>(&q);
-      for (int i = 0; i < kVec && v + i < length; ++i) e[i] = x[v + i];
+  constexpr int kAhead = 4;                               // loads of a thread under way
+  for (int v0 = warp * stretch + lane * kVec; v0 < (warp + 1) * stretch; v0 += kAhead * 32 * kVec) {
+    uint4 q[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int v = v0 + a * 32 * kVec;
+      q[a] = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
+      if (v >= (warp + 1) * stretch) continue;
+      if (whole && v + kVec <= length) {
+        q[a] = *reinterpret_cast<const uint4*>(x + v);
+      } else {
+        T e[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) e[i] = v + i < length ? x[v + i] : from_f32<T>(__int_as_float(0x7fffffff));
+        q[a] = *reinterpret_cast<const uint4*>(e);
+      }
     }
-    s_data[v / kVec] = q;
-    r.vec(v, [&](uint32_t k, int) {
-      high = max(high, k);
-      low = min(low, k);
-    });
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int v = v0 + a * 32 * kVec;
+      if (v >= (warp + 1) * stretch) continue;
+      const uint32_t w[4] = {q[a].x, q[a].y, q[a].z, q[a].w};
+      uint32_t keys[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        keys[e] = Key<T>::of(sizeof(T) == 4 ? w[e & 3] : e & 1 ? w[e / 2 % 4] & 0xffff0000u : w[e / 2 % 4] << 16);
+        high = max(high, keys[e]);
+        low = min(low, keys[e] > Key<T>::kMinusInf ? keys[e] : 0xffffffffu);
+      }
+      s_data[v / kVec] = Key<T>::pack(keys);
+    }
   }
   // the largest lane maxima of every warp
   const int warps = min(r.blocks * kWarps, (V + stretch - 1) / stretch);     // that have tokens
-  const int draws = max(2, (2 * top_k + warps - 1) / warps);
+  const int draws = (2 * top_k + warps - 1) / warps;
   const bool few = top_k > 0 && top_k < V && top_k <= kFew && draws <= 32;
   if (few) {
     uint32_t m = high;
@@ -416,24 +488,29 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits
   if (few) {                                              // the k-th largest of them
     const int each = min(kWarps, warps) * draws, n = warps * draws;
     if (tid < n) s.all_tops[tid] = r.blocks > 1 ? peer32(&s.tops[tid % each], tid / each) : s.tops[tid];
+    if (tid < 4) s.all_tops[n + tid] = 0;
     __syncthreads();
     if (tid < n) {
       const uint32_t mine = s.all_tops[tid];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t t = s.all_tops[j];
-        rank += t > mine || (t == mine && j < tid);
+      int above = 0, equal = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; j += 4) {
+        const uint4 t = *reinterpret_cast<const uint4*>(&s.all_tops[j]);
+        above += (t.x > mine) + (t.y > mine) + (t.z > mine) + (t.w > mine);
+        equal += (t.x == mine) + (t.y == mine) + (t.z == mine) + (t.w == mine);
       }
-      if (rank == top_k - 1) s.tau = mine;
+      if (mine > 0 && above < top_k && top_k <= above + equal) s.tau = mine;
     }
   }
   r.sync();
-  const uint32_t tau = s.tau;
+  const uint32_t reach = max(s.tau, Key<T>::kMinusInf + 1);
   r.best = best;
-  r.top = value_of(best);
-  r.rate = 92.332482616893656 / static_cast<double>(temperature);          // 64 log2 e
+  r.top = Key<T>::value(best);
+  const double rate = 369.32993046757462 / static_cast<double>(temperature);   // 256 log2 e
+  r.rate = static_cast<float>(rate);
+  r.rate_low = static_cast<float>(rate - static_cast<double>(r.rate));
 
-  if (best <= kMinusInf) {                                // nothing to draw from
+  if (best <= Key<T>::kMinusInf) {                                // nothing to draw from
     if (tid == 0 && r.rank == 0) ids[b] = 0, probs[b] = 0.f;
     return;
   }
@@ -444,27 +521,36 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits
   }
   const u64 least_mass = min_p >= 1.f ? kOne : min_p > 0.f ? static_cast<u64>(ceil(static_cast<double>(min_p) * kOne)) : 0;
   const u64 u = fraction(p.uniform[b]), share = fraction(top_p);
-  uint32_t from = kMinusInf + 1;
+  uint32_t from = Key<T>::kMinusInf + 1;
   bool listed = false;
   unsigned n = 0;
-  if (few) {
-    n = collect(r, [&](uint32_t k, int) { return k >= tau; });
+  if (few) {                                              // straight into the first block's list
+    const uint32_t count = map_to_cta(smem_u32(&s.count), 0), list = map_to_cta(smem_u32(s.list), 0);
+    r.each([&](uint32_t k, int i) {
+      if (k < reach) return;
+      unsigned at;
+      asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
+      if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(token(k, i)) : "memory");
+    });
+    r.sync();
+    n = r.rank == 0 ? s.count : peer32(&s.count, 0);
     listed = n <= kList;
+    r.sync();
   }
   if (listed) {
-    // everything that top-k may keep is in every block's list
     if (r.rank == 0) {
       const u64 mine = tid < n ? s.list[tid] : 0;
       const uint32_t key = mine >> 32;
       int rank = 0, greater = 0;
+      if (tid < 4) s.list[n + tid] = 0;                     // behind everything
+      __syncthreads();
       if (tid < n) {
-        for (int j = 0; j < n; ++j) {
-          const u64 t = s.list[j];
-          rank += t > mine;
-          greater += static_cast<uint32_t>(t >> 32) > key;
-        }
-        s.mass[tid] = greater < top_k ? r.mass(key) : 0;
-        s.sorted[rank] = s.mass[tid];
+        pairs(n, [&](int j) {
+          const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(&s.list[j]);
+          rank += (t.x > mine) + (t.y > mine);
+          greater += (static_cast<uint32_t>(t.x >> 32) > key) + (static_cast<uint32_t>(t.y >> 32) > key);
+        });
+        s.sorted[rank] = greater < top_k ? r.mass(key) : 0;
       }
       __syncthreads();
       const u64 w = tid < n ? s.sorted[tid] : 0;
@@ -475,6 +561,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits
       const u64 kept = tid < n ? s.sorted[rank] : 0;
       __syncthreads();
       if (tid < n) s.mass[tid] = kept;
+      if (tid < 4) s.mass[n + tid] = 0;
       block_before(kept, s.sums);
       const u64 left = all_sums(s.sums);
       __syncthreads();
@@ -482,8 +569,10 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits
       if (kept > 0) {
         u64 before = 0;
         const uint32_t at = static_cast<uint32_t>(mine);                   // ~index
-        for (int j = 0; j < n; ++j)
-          if (static_cast<uint32_t>(s.list[j]) > at) before += s.mass[j];
+        pairs(n, [&](int j) {
+          const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(&s.list[j]), m = *reinterpret_cast<const ulonglong2*>(&s.mass[j]);
+          before += (static_cast<uint32_t>(t.x) > at ? m.x : 0) + (static_cast<uint32_t>(t.y) > at ? m.y : 0);
+        });
         const u64 target = __umul64hi(u, left);
         if (before <= target && target < before + kept) {
           ids[b] = static_cast<int>(~at);
@@ -491,16 +580,14 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(const T* logits
         }
       }
     }
-    if (r.blocks > 1) r.sync();
     return;
   }
   if (top_k > 0 && top_k < V) from = max(from, static_cast<uint32_t>(border<false>(r, least, best, static_cast<u64>(top_k - 1)) >> 32));
   u64 last = token(from, 0x7fffffff);                     // the last token that stays
   if (top_p < 1.f) last = border<true>(r, max(from, least), best, share);
   auto held = [&](uint32_t k, int i) -> u64 {
-    if (token(k, i) < last) return 0;
     const u64 w = r.mass(k);
-    return w < least_mass ? 0 : w;
+    return token(k, i) < last || w < least_mass ? 0 : w;
   };
   u64 own = 0;
   r.each([&](uint32_t k, int i) { own += held(k, i); });
@@ -534,19 +621,16 @@ int sm_count() {
   return n;
 }
 
-template <typename T>
-cudaError_t launch_one(const void* logits, long long ld, int B, int V, const cd_sample& p, int64_t* ids, float* probs, cudaStream_t stream) {
-  constexpr auto kKernel = sample_tokens_kernel<T>;
-  constexpr int kVec = Row<T>::kVec;
-  // as many blocks a row as its size asks for, and more while the device has SMs without one and a block has 4 096 tokens
-  int blocks = 1;
-  while (static_cast<long long>(V) * sizeof(T) > static_cast<long long>(blocks) * kSliceBytes) blocks *= 2;
-  while (blocks < kMostBlocks && 2LL * blocks * B <= sm_count() && V / (2 * blocks) >= 4096) blocks *= 2;
+template <typename T, int kThreads>
+cudaError_t launch_blocks(int blocks, const T* logits, long long ld, int B, int V, const cd_sample& p, long long* ids, float* probs,
+                          cudaStream_t stream) {
+  constexpr auto kKernel = sample_tokens_kernel<T, kThreads>;
+  constexpr int kVec = Row<T, kThreads>::kVec, kWarps = kThreads / 32;
   const int least = 32 * kVec;                            // of a warp: 16 bytes a lane
   int stretch = (V + blocks * kWarps - 1) / (blocks * kWarps);
   stretch = stretch < least ? least : (stretch + kVec - 1) / kVec * kVec;
-  const int slice = stretch * kWarps, bytes = (sizeof(Shared) + 15) / 16 * 16 + slice * static_cast<int>(sizeof(T));
-  cudaError_t e = allow_smem<kKernel>(bytes);
+  const int slice = stretch * kWarps, bytes = (sizeof(Shared<kThreads>) + 15) / 16 * 16 + slice * static_cast<int>(sizeof(T));
+  const cudaError_t e = allow_smem<kKernel>(bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, B);
@@ -561,7 +645,22 @@ cudaError_t launch_one(const void* logits, long long ld, int B, int V, const cd_
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = blocks > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kKernel, static_cast<const T*>(logits), ld, V, slice, stretch, p, reinterpret_cast<long long*>(ids), probs);
+  return cudaLaunchKernelEx(&cfg, kKernel, logits, ld, V, slice, stretch, p, ids, probs);
+}
+
+// As many blocks a row as its size asks for, and more while there is an SM for each and 4 096 tokens. us, 1 / 2 / 4 / 8 blocks of 512
+// threads: 1 x 32 000 11.7 / 10.8 / 9.7 / 9.8, 32 x 100 000 22.6 / 17.0 / 14.8 / 19.3 (two an SM), nucleus of 64 x 100 000
+// - / 68 / 91 / 135. Long shares take 1 024 threads: the nucleus 61, 256 x 32 000 in 32 bits 57 (62); short ones do not (1 x 32 000,
+// 4 blocks: 11.6).
+template <typename T>
+cudaError_t launch_one(const void* logits, long long ld, int B, int V, const cd_sample& p, int64_t* ids, float* probs, cudaStream_t stream) {
+  int blocks = 1;
+  while (static_cast<long long>(V) * sizeof(T) > static_cast<long long>(blocks) * kSliceBytes) blocks *= 2;
+  while (blocks < kMostBlocks && 2LL * blocks * B <= sm_count() && V / (2 * blocks) >= 4096) blocks *= 2;
+  const T* x = static_cast<const T*>(logits);
+  long long* to = reinterpret_cast<long long*>(ids);
+  return V / blocks > 16384 ? launch_blocks<T, 1024>(blocks, x, ld, B, V, p, to, probs, stream)
+                            : launch_blocks<T, 512>(blocks, x, ld, B, V, p, to, probs, stream);
 }
 
 }  // namespace
