@@ -1,9 +1,15 @@
 // Cuts a paged cache back to `keep` rows per (layer, sequence, KV head): the newest `recent` rows stay, then those of the largest
 // accumulated attention weight, ties by the lowest row. Of the rows that stay, those behind row `keep` move into the places of those
-// given up in front of it, in order, so nothing is read that has been written and only the moved rows are touched.
+// given up in front of it, in order, so nothing is read that has been written and only the moved rows are touched: 16 D bytes
+// each (read and written, keys and values), beside 8 bytes of weight and position of every row.
 //
-// One block a (layer, sequence, head). The keep-th largest key is found digit by digit (histograms of eight bits, keys read again
-// from L2), then one walk in row order gives every row its fate and the movers and holes their ranks.
+// A block a (layer, sequence, head). Keys (the weights' order as unsigned numbers) are read once into shared memory. The keep-th
+// largest is found by histograms of 11, 11 and 10 bits; of the first, sign, exponent and two bits, lognormal weights use some
+// forty bins, which keeps warps from queueing at a few. Then warps walk their stretches of rows by ballots: ties, fates (a
+// bit a row), and the ranks of holes and movers, whose lists take the keys' place.
+//
+// Few pairs of long caches take several blocks each, a cluster: all find the same fates (reading 8 bytes a row again costs less than
+// telling one another) and move a share of the rows, behind a barrier, since weights may be replaced in place.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "checks.cuh"
@@ -14,15 +20,20 @@ namespace cdeep {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kBins = 2048;
+constexpr int kMostBlocks = 8;            // of a pair
+constexpr int kSmallRows = 4096;          // up to here blocks of 256 threads, several an SM
+constexpr int kHeldRows = 52 * 1024;      // beyond, keys are read again and lists lie in the workspace
 
 struct Args {
   cd_paged c;
   long long stride_l;
   cd_evict e;
   int B, hkv, D;
-  int* lists;            // [pairs][2][most]: moved rows, holes
-  int most;
+  int shift;              // log2 of the page, or -1
+  int blocks;             // of a pair
+  int* lists;             // [pairs][rows + words]: where keys are not held
+  int rows, half, words;  // of a sequence at most; of a list at most; of the fates' bits
   int* status;
 };
 
@@ -33,111 +44,242 @@ __device__ __forceinline__ uint32_t key_of(float w, bool newest) {
   return newest ? 0xffffffffu : k;
 }
 
-__global__ void __launch_bounds__(kThreads) evict_rows_kernel(Args a) {
-  __shared__ unsigned s_hist[256];
-  __shared__ int s_scan[3][kThreads / 32];
+// Sum over the warps ahead of this one, and over all, of a number that every lane of a warp has.
+template <int kWarps>
+__device__ __forceinline__ int warps_before(int v, int* s, int& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+  if (lane == 0) s[warp] = v;
+  __syncthreads();
+  const int x = lane < kWarps ? s[lane] : 0;
+  all = __reduce_add_sync(0xffffffffu, x);
+  return __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+}
+
+template <int kThreads, bool kHeld>
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 5 : 1) evict_rows_kernel(const Args a) {
+  constexpr int kWarps = kThreads / 32, kOwn = kBins / kThreads;
+  extern __shared__ __align__(16) unsigned s_dyn[];
+  __shared__ int s_warps[kWarps];
   __shared__ unsigned s_digit, s_left;
+  unsigned* hist = s_dyn;
   griddep_wait();
   griddep_launch_dependents();
-  const int h = blockIdx.x % a.hkv, b = blockIdx.x / a.hkv % a.B, layer = blockIdx.x / (a.hkv * a.B);
-  const int rows = a.c.width * a.c.page, keep = a.e.keep;
-  const int n = min(a.c.lengths[b], rows);
-  const long long base = static_cast<long long>(blockIdx.x) * rows;
+  const int pair = blockIdx.x / a.blocks, rank = blockIdx.x - pair * a.blocks;
+  const int h = pair % a.hkv, b = pair / a.hkv % a.B, layer = pair / (a.hkv * a.B);
+  const int keep = a.e.keep, n = min(a.c.lengths[b], a.rows);
+  const long long base = static_cast<long long>(pair) * a.rows;
   const float* w = a.c.weights + base;
   const int* pos = a.e.row_positions + base;
   float* w_out = a.e.weights_out + base;
   int* pos_out = a.e.row_positions_out + base;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool in_place = w_out == w;
-  if (n <= keep) {
+  if (n <= keep) {                        // the same for all blocks of the pair
     if (!in_place)
-      for (int i = tid; i < n; i += kThreads) w_out[i] = w[i], pos_out[i] = pos[i];
+      for (int i = rank * kThreads + tid; i < n; i += a.blocks * kThreads) w_out[i] = w[i], pos_out[i] = pos[i];
     return;
   }
+  int* own = a.lists + (static_cast<long long>(pair) * a.blocks + rank) * (a.rows + a.words);
+  unsigned* keys = kHeld ? s_dyn + kBins : nullptr;
+  int* lists = kHeld ? reinterpret_cast<int*>(keys) : own;                 // behind the fates: holes, then movers
+  unsigned* fates = kHeld ? keys + a.rows : reinterpret_cast<unsigned*>(own + a.rows);
   const long long oldest = static_cast<long long>(a.e.positions[b]) - a.e.recent;
-  auto key = [&](int i) { return key_of(w[i], pos[i] >= oldest); };
+  auto key = [&](int i) -> unsigned {
+    if constexpr (kHeld) return keys[i];
+    return key_of(w[i], pos[i] >= oldest);
+  };
+  if constexpr (kHeld) {
+    constexpr int kAhead = 4;
+    for (int i0 = tid; i0 < n; i0 += kAhead * kThreads) {
+      float wi[kAhead];
+      int pi[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * kThreads;
+        wi[x] = i < n ? w[i] : 0.f;
+        pi[x] = i < n ? pos[i] : 0;
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * kThreads;
+        if (i < n) keys[i] = key_of(wi[x], pi[x] >= oldest);
+      }
+    }
+  }
 
+  // the keep-th largest key, and how many of those equal to it stay
   unsigned prefix = 0, left = keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int i = tid; i < bins; i += kThreads) hist[i] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += kThreads) {
       const unsigned k = key(i);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[k >> shift & 255], 1u);
+      if (pass == 0 || (k ^ prefix) >> (shift + (pass == 1 ? 11 : 10)) == 0) atomicAdd(&hist[k >> shift & (bins - 1)], 1u);
     }
     __syncthreads();
-    if (tid == 0) {
-      int d = 255;
-      while (d > 0 && s_hist[d] < left) left -= s_hist[d--];
-      s_digit = d;
-      s_left = left;
+    // thread 0 has the largest bins
+    unsigned count[kOwn], sum = 0;
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x) {
+      const int bin = bins - 1 - (tid * kOwn + x);
+      count[x] = bin >= 0 ? hist[bin] : 0;
+      sum += count[x];
+    }
+    unsigned upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    int all;
+    unsigned before = warps_before<kWarps>(static_cast<int>(__shfl_sync(0xffffffffu, upto, 31)), s_warps, all) + upto - sum;
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x) {
+      if (before < left && left <= before + count[x]) {
+        s_digit = bins - 1 - (tid * kOwn + x);
+        s_left = left - before;
+      }
+      before += count[x];
     }
     __syncthreads();
     prefix |= s_digit << shift;
     left = s_left;
   }
 
-  // Rows in order, a tile at a time: counts of equal keys, holes and movers ahead of each.
-  int* moved = a.lists + static_cast<long long>(blockIdx.x) * 2 * a.most;
-  int* holes = moved + a.most;
-  int seen[3] = {0, 0, 0};
-  auto ranks = [&](bool flag, int which) {                // flags ahead of this thread's, all tiles
-    const unsigned vote = __ballot_sync(0xffffffffu, flag);
-    if (lane == 0) s_scan[which][warp] = __popc(vote);
-    __syncthreads();
-    int before = seen[which], total = 0;
-    for (int x = 0; x < kThreads / 32; ++x) {
-      const int c = s_scan[which][x];
-      if (x < warp) before += c;
-      total += c;
-    }
-    seen[which] += total;
-    __syncthreads();
-    return before + __popc(vote & ((1u << lane) - 1));
-  };
-  for (int t = 0; t < n; t += kThreads) {
-    const int i = t + tid;
+  // fates, a bit a row: a warp has a stretch of whole words
+  const int words = (n + 31) / 32, stretch = (words + kWarps - 1) / kWarps;
+  const int from = min(words, warp * stretch), to = min(words, from + stretch);
+  int ties = 0, all;
+  for (int x = from; x < to; ++x) {
+    const int i = x * 32 + lane;
+    ties += __popc(__ballot_sync(0xffffffffu, i < n && key(i) == prefix));
+  }
+  int tie = warps_before<kWarps>(ties, s_warps, all);
+  int holes = 0, movers = 0;
+  const unsigned below = (1u << lane) - 1;
+  for (int x = from; x < to; ++x) {
+    const int i = x * 32 + lane;
     const unsigned k = i < n ? key(i) : 0;
-    const bool tie = i < n && k == prefix;
-    const int tie_rank = ranks(tie, 0);
-    const bool stays = i < n && (k > prefix || (tie && tie_rank < static_cast<int>(left)));
-    const bool hole = i < keep && !stays, mover = i >= keep && stays;
-    const int hole_rank = ranks(hole, 1), mover_rank = ranks(mover, 2);
-    if (hole) holes[hole_rank] = i;
-    if (mover) moved[mover_rank] = i;
-    if (!in_place && i < keep && stays) w_out[i] = w[i], pos_out[i] = pos[i];
+    const unsigned equal = __ballot_sync(0xffffffffu, i < n && k == prefix);
+    const bool stays = i < n && (k > prefix || (k == prefix && tie + __popc(equal & below) < static_cast<int>(left)));
+    tie += __popc(equal);
+    const unsigned bits = __ballot_sync(0xffffffffu, stays);
+    if (lane == 0) fates[x] = bits;
+    holes += __popc(__ballot_sync(0xffffffffu, i < keep && !stays));
+    movers += __popc(__ballot_sync(0xffffffffu, i >= keep && stays));
+    if (!in_place && i < keep && stays && x % a.blocks == rank) w_out[i] = w[i], pos_out[i] = pos[i];
   }
-  __syncthreads();
-  const int moves = seen[2];
+  int moves;
+  int hole = warps_before<kWarps>(holes, s_warps, moves);
+  int mover = warps_before<kWarps>(movers, s_warps, moves);
+  __syncthreads();                        // every key has been read
+  for (int x = from; x < to; ++x) {
+    const int i = x * 32 + lane;
+    const unsigned bits = fates[x], front = i < keep && i < n ? 1u : 0u;
+    const unsigned is_hole = __ballot_sync(0xffffffffu, front && !(bits >> lane & 1));
+    const unsigned is_mover = __ballot_sync(0xffffffffu, !front && (bits >> lane & 1));
+    if (is_hole >> lane & 1) lists[hole + __popc(is_hole & below)] = i;
+    if (is_mover >> lane & 1) lists[a.half + mover + __popc(is_mover & below)] = i;
+    hole += __popc(is_hole);
+    mover += __popc(is_mover);
+  }
+  if (a.blocks > 1) {
+    cluster_sync_all();                   // every block has read every weight
+  } else {
+    __syncthreads();
+  }
+
+  // the rows, a warp several at a time: its lanes take 16 bytes each, of keys and then of values
   const int* table = a.c.table + b * a.c.table_stride;
-  for (int x = tid; x < moves; x += kThreads) {
-    w_out[holes[x]] = w[moved[x]];
-    pos_out[holes[x]] = pos[moved[x]];
-  }
-  const int pieces = a.D / 8;                             // 16 bytes each
   const long long at = layer * a.stride_l + h * a.c.stride_h;
-  uint4* pools[2] = {reinterpret_cast<uint4*>(a.c.k), reinterpret_cast<uint4*>(a.c.v)};
-  for (int x = tid; x < 2 * moves * pieces; x += kThreads) {
-    const int row = x / (2 * pieces), piece = x % pieces, which = x / pieces % 2;
-    const int src = moved[row], dst = holes[row], ps = table[src / a.c.page], pd = table[dst / a.c.page];
-    if (ps < 0 || ps >= a.c.pages || pd < 0 || pd >= a.c.pages) {
-      atomicMax(a.status, kStatusBounds);
-      continue;
+  const int pieces = a.D / 8;
+  auto place = [&](int row) -> long long {
+    const int page = a.shift >= 0 ? row >> a.shift : row / a.c.page, within = row - page * a.c.page, id = table[page];
+    if (id >= 0 && id < a.c.pages) return (at + id * a.c.stride_p + within * a.c.stride_t) / 8;
+    atomicMax(a.status, kStatusBounds);
+    return -1;
+  };
+  uint4* const k = static_cast<uint4*>(a.c.k);
+  uint4* const v = static_cast<uint4*>(a.c.v);
+  constexpr int kAhead = 4;
+  for (int m0 = (rank * kWarps + warp) * kAhead; m0 < moves; m0 += a.blocks * kWarps * kAhead) {
+    // lane x: row m0 + x
+    const int m = m0 + (lane & (kAhead - 1));
+    long long src = -1, dst = -1;
+    if (m < moves) {
+      const int s = lists[a.half + m], d = lists[m];
+      src = place(s);
+      dst = place(d);
+      if (lane < kAhead) {
+        w_out[d] = w[s];
+        pos_out[d] = pos[s];
+      }
     }
-    pools[which][(at + pd * a.c.stride_p + dst % a.c.page * a.c.stride_t) / 8 + piece] =
-        pools[which][(at + ps * a.c.stride_p + src % a.c.page * a.c.stride_t) / 8 + piece];
+    if (src < 0 || dst < 0) src = dst = -1;
+    for (int p0 = 0; p0 < 2 * pieces; p0 += 32) {
+      const int p = p0 + lane;
+      uint4* const pool = p < pieces ? k : v;
+      const int x = p < pieces ? p : p - pieces;
+      uint4 held[kAhead];
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {
+        const long long s = __shfl_sync(0xffffffffu, src, r);
+        if (p < 2 * pieces && s >= 0) held[r] = pool[s + x];
+      }
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r) {
+        const long long d = __shfl_sync(0xffffffffu, dst, r);
+        if (p < 2 * pieces && d >= 0) pool[d + x] = held[r];
+      }
+    }
   }
+}
+
+int sm_count() {
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 148;
+  return n;
+}
+
+template <int kThreads, bool kHeld>
+cudaError_t launch_one(const Args& a, int pairs, cudaStream_t stream) {
+  constexpr auto kKernel = evict_rows_kernel<kThreads, kHeld>;
+  const int bytes = 4 * (kBins + (kHeld ? a.rows + a.words : 0));
+  const cudaError_t e = allow_smem<kKernel>(bytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.blocks * pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.blocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.blocks > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kKernel, a);
+}
+
+// Blocks of a pair: more than one where there are SMs without and 128 moved rows for each.
+int blocks_of(long long pairs, int rows, int keep) {
+  const int most = rows - keep < keep ? rows - keep : keep;
+  int blocks = 1;
+  while (blocks < kMostBlocks && 2 * blocks * pairs <= sm_count() && most >= 256 * blocks) blocks *= 2;
+  return blocks;
 }
 
 }  // namespace
 
-int evict_most(int width, int page, int keep) {
-  const long long rows = static_cast<long long>(width) * page;
-  return rows <= keep ? 0 : static_cast<int>(rows - keep < keep ? rows - keep : keep);
-}
-
 size_t evict_rows_workspace_bytes(int layers, int B, int hkv, int page, int width, int keep) {
-  return sizeof(int) * 2 * layers * B * hkv * evict_most(width, page, keep);
+  const long long rows = static_cast<long long>(width) * page, pairs = static_cast<long long>(layers) * B * hkv;
+  if (rows <= kHeldRows || rows <= keep) return 0;
+  return sizeof(int) * pairs * blocks_of(pairs, static_cast<int>(rows), keep) * (rows + (rows + 31) / 32);
 }
 
 cudaError_t launch_evict_rows(const cd_paged& c, const cd_evict& e, int layers, long long stride_l, int B, int hkv, int D, void* ws,
@@ -149,10 +291,18 @@ cudaError_t launch_evict_rows(const cd_paged& c, const cd_evict& e, int layers, 
   a.B = B;
   a.hkv = hkv;
   a.D = D;
+  a.shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (c.page == 1 << s) a.shift = s;
+  const int pairs = layers * B * hkv;
+  a.rows = c.width * c.page;
+  a.half = a.rows / 2;                    // there are as many movers as holes
+  a.words = (a.rows + 31) / 32;
+  a.blocks = a.rows <= e.keep ? 1 : blocks_of(pairs, a.rows, e.keep);
   a.lists = static_cast<int*>(ws);
-  a.most = evict_most(c.width, c.page, e.keep);
   a.status = status;
-  return launch_kernel(evict_rows_kernel, dim3(layers * B * hkv), dim3(kThreads), 0, stream, a);
+  if (a.rows <= kSmallRows) return launch_one<256, true>(a, pairs, stream);
+  return a.rows <= kHeldRows ? launch_one<1024, true>(a, pairs, stream) : launch_one<1024, false>(a, pairs, stream);
 }
 
 }  // namespace cdeep

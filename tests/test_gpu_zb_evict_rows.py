@@ -66,6 +66,13 @@ def test_layers_and_long():
     _run([40 + i for i in range(50)], 8, 64, 16, 41, 4, seed=6)
 
 
+def test_rows_beyond_what_a_block_holds():
+    """Tables of more than 53 248 rows: keys are read again, lists lie in the workspace; also with several blocks a pair."""
+    _run([60000, 700], 1, 64, 256, 650, 100, seed=7, width=256)
+    _run([3000, 60000, 64], 2, 8, 64, 2000, 0, seed=8, width=1024, in_place=False)
+    _run([60000], 1, 64, 64, 30000, 5, seed=9, width=1000, ties=True, order="rows")
+
+
 def test_odd_weights():
     """Equal ones, zeros of both signs, negative, infinite and NaN."""
     shape = (2, 1, 160)
