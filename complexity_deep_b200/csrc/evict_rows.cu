@@ -22,7 +22,8 @@ namespace {
 
 constexpr int kBins = 2048;
 constexpr int kMostBlocks = 8;            // of a pair
-constexpr int kSmallRows = 4096;          // up to here blocks of 256 threads, several an SM
+constexpr int kSmallRows = 4096;          // up to here small blocks, several an SM
+constexpr int kSmallThreads = 128;
 constexpr int kHeldRows = 52 * 1024;      // beyond, keys are read again and lists lie in the workspace
 
 struct Args {
@@ -57,11 +58,11 @@ __device__ __forceinline__ int warps_before(int v, int* s, int& all) {
 }
 
 template <int kThreads, bool kHeld>
-__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 5 : 1) evict_rows_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, kThreads == kSmallThreads ? 7 : 1) evict_rows_kernel(const Args a) {
   constexpr int kWarps = kThreads / 32, kOwn = kBins / kThreads;
   extern __shared__ __align__(16) unsigned s_dyn[];
   __shared__ int s_warps[kWarps];
-  __shared__ unsigned s_digit, s_left;
+  __shared__ unsigned s_digit, s_left, s_equal;
   unsigned* hist = s_dyn;
   griddep_wait();
   griddep_launch_dependents();
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 5 : 1) evict_rows_
     return key_of(w[i], pos[i] >= oldest);
   };
   if constexpr (kHeld) {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     for (int i0 = tid; i0 < n; i0 += kAhead * kThreads) {
       float wi[kAhead];
       int pi[kAhead];
@@ -113,21 +114,31 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 5 : 1) evict_rows_
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < bins; i += kThreads) hist[i] = 0;
+    for (int i = tid; i < bins / 4; i += kThreads) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     for (int i = tid; i < n; i += kThreads) {
       const unsigned k = key(i);
       if (pass == 0 || (k ^ prefix) >> (shift + (pass == 1 ? 11 : 10)) == 0) atomicAdd(&hist[k >> shift & (bins - 1)], 1u);
     }
     __syncthreads();
-    // thread 0 has the largest bins
-    unsigned count[kOwn], sum = 0;
+    // thread 0 has the largest bins; every thread neighbouring ones, read four (two) at a time
+    const int own = bins / kThreads, low = bins - (tid + 1) * own;
+    unsigned count[kOwn] = {}, sum = 0;                     // the largest first
 #pragma unroll
-    for (int x = 0; x < kOwn; ++x) {
-      const int bin = bins - 1 - (tid * kOwn + x);
-      count[x] = bin >= 0 ? hist[bin] : 0;
-      sum += count[x];
+    for (int x = 0; x < kOwn; x += kOwn < 4 ? kOwn : 4) {
+      if constexpr (kOwn < 4) {
+        count[0] = hist[low + own - 1];
+        if (own > 1) count[1] = hist[low];
+      } else if (x < own) {
+        const uint4 c = *reinterpret_cast<const uint4*>(hist + low + own - 4 - x);
+        count[x] = c.w;
+        count[x + 1] = c.z;
+        count[x + 2] = c.y;
+        count[x + 3] = c.x;
+      }
     }
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x) sum += count[x];
     unsigned upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -139,8 +150,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 5 : 1) evict_rows_
 #pragma unroll
     for (int x = 0; x < kOwn; ++x) {
       if (before < left && left <= before + count[x]) {
-        s_digit = bins - 1 - (tid * kOwn + x);
+        s_digit = low + own - 1 - x;
         s_left = left - before;
+        s_equal = count[x];
       }
       before += count[x];
     }
@@ -149,42 +161,74 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 5 : 1) evict_rows_
     left = s_left;
   }
 
-  // fates, a bit a row: a warp has a stretch of whole words
+  // fates, a bit a row: a warp has a stretch of whole words; where only some of the equal rows stay, their order counts
   const int words = (n + 31) / 32, stretch = (words + kWarps - 1) / kWarps;
   const int from = min(words, warp * stretch), to = min(words, from + stretch);
-  int ties = 0, all;
-  for (int x = from; x < to; ++x) {
-    const int i = x * 32 + lane;
-    ties += __popc(__ballot_sync(0xffffffffu, i < n && key(i) == prefix));
-  }
-  int tie = warps_before<kWarps>(ties, s_warps, all);
-  int holes = 0, movers = 0;
   const unsigned below = (1u << lane) - 1;
+  const bool some = s_equal != left;
+  int tie = 0;
+  if (some) {
+    int ties = 0, all;
+    for (int x = from; x < to; ++x) {
+      const int i = x * 32 + lane;
+      ties += __popc(__ballot_sync(0xffffffffu, i < n && key(i) == prefix));
+    }
+    tie = warps_before<kWarps>(ties, s_warps, all);
+  }
+#pragma unroll 4
   for (int x = from; x < to; ++x) {
     const int i = x * 32 + lane;
     const unsigned k = i < n ? key(i) : 0;
-    const unsigned equal = __ballot_sync(0xffffffffu, i < n && k == prefix);
-    const bool stays = i < n && (k > prefix || (k == prefix && tie + __popc(equal & below) < static_cast<int>(left)));
-    tie += __popc(equal);
+    bool stays = i < n && k >= prefix;
+    if (some) {
+      const unsigned equal = __ballot_sync(0xffffffffu, i < n && k == prefix);
+      if (k == prefix && tie + __popc(equal & below) >= static_cast<int>(left)) stays = false;
+      tie += __popc(equal);
+    }
     const unsigned bits = __ballot_sync(0xffffffffu, stays);
     if (lane == 0) fates[x] = bits;
-    holes += __popc(__ballot_sync(0xffffffffu, i < keep && !stays));
-    movers += __popc(__ballot_sync(0xffffffffu, i >= keep && stays));
-    if (!in_place && i < keep && stays && x % a.blocks == rank) w_out[i] = w[i], pos_out[i] = pos[i];
   }
-  int moves;
-  int hole = warps_before<kWarps>(holes, s_warps, moves);
-  int mover = warps_before<kWarps>(movers, s_warps, moves);
   __syncthreads();                        // every key has been read
-  for (int x = from; x < to; ++x) {
-    const int i = x * 32 + lane;
-    const unsigned bits = fates[x], front = i < keep && i < n ? 1u : 0u;
-    const unsigned is_hole = __ballot_sync(0xffffffffu, front && !(bits >> lane & 1));
-    const unsigned is_mover = __ballot_sync(0xffffffffu, !front && (bits >> lane & 1));
-    if (is_hole >> lane & 1) lists[hole + __popc(is_hole & below)] = i;
-    if (is_mover >> lane & 1) lists[a.half + mover + __popc(is_mover & below)] = i;
-    hole += __popc(is_hole);
-    mover += __popc(is_mover);
+  if (!in_place) {                        // rows that stay where they are; those that do not are filled below
+    constexpr int kAhead = 4;
+    for (int i0 = rank * kThreads + tid; i0 < keep; i0 += a.blocks * kThreads * kAhead) {
+      float wi[kAhead];
+      int pi[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = min(i0 + x * a.blocks * kThreads, keep - 1);
+        wi[x] = w[i];
+        pi[x] = pos[i];
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int i = i0 + x * a.blocks * kThreads;
+        if (i < keep && (fates[i >> 5] >> (i & 31) & 1)) w_out[i] = wi[x], pos_out[i] = pi[x];
+      }
+    }
+  }
+  // holes and movers in order, a thread a word
+  int seen_holes = 0, moves = 0;
+  for (int x0 = 0; x0 < words; x0 += kThreads) {
+    const int x = x0 + tid, ahead = keep - x * 32;        // rows of the word in front of row `keep`
+    const unsigned bits = x < words ? fates[x] : 0, front = ahead >= 32 ? ~0u : ahead <= 0 ? 0u : (1u << ahead) - 1;
+    unsigned hole = x < words ? ~bits & front : 0, mover = bits & ~front;
+    const int counts = __popc(hole) | __popc(mover) << 16;                 // of a warp at most 1 024 each
+    int upto = counts;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    const int warp_counts = __shfl_sync(0xffffffffu, upto, 31);
+    upto -= counts;
+    int all_holes, all_movers;
+    int to_hole = seen_holes + warps_before<kWarps>(warp_counts & 0xffff, s_warps, all_holes) + (upto & 0xffff);
+    int to_mover = moves + warps_before<kWarps>(warp_counts >> 16, s_warps, all_movers) + (upto >> 16);
+    for (; hole; hole &= hole - 1) lists[to_hole++] = x * 32 + __ffs(hole) - 1;
+    for (; mover; mover &= mover - 1) lists[a.half + to_mover++] = x * 32 + __ffs(mover) - 1;
+    seen_holes += all_holes;
+    moves += all_movers;
   }
   if (a.blocks > 1) {
     cluster_sync_all();                   // every block has read every weight
@@ -301,7 +345,7 @@ cudaError_t launch_evict_rows(const cd_paged& c, const cd_evict& e, int layers, 
   a.blocks = a.rows <= e.keep ? 1 : blocks_of(pairs, a.rows, e.keep);
   a.lists = static_cast<int*>(ws);
   a.status = status;
-  if (a.rows <= kSmallRows) return launch_one<256, true>(a, pairs, stream);
+  if (a.rows <= kSmallRows) return launch_one<kSmallThreads, true>(a, pairs, stream);
   return a.rows <= kHeldRows ? launch_one<1024, true>(a, pairs, stream) : launch_one<1024, false>(a, pairs, stream);
 }
 
