@@ -10,11 +10,14 @@
 //
 // Work is cut into tiles of 64 rows; all tiles of all (sequence, KV head) pairs stand in one line, of which every block takes an equal
 // stretch, whatever the lengths are. A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
-// block, which the second kernel adds in order (results do not depend on timing). A warp feeds tiles to the ring with TMA (a
+// block, which a second kernel adds in order (results do not depend on timing). A warp feeds tiles to the ring with TMA (a
 // box per page, 128-byte swizzle), four warps take 16 rows of a tile each, with a running maximum and sum of their own.
 //
+// Short caches take a cluster of blocks a pair instead (kCluster), whose sums meet in shared memory: one launch, no workspace to meet
+// in, and no line to find one's place in.
+//
 // The share of a row in its softmax is known only when the pair's maximum and sum are: where weights are asked for, scores are
-// left in the workspace and the second kernel turns them into shares.
+// left in the workspace and the second kernel turns them into shares (clusters do so themselves, when their sums have met).
 //
 // A step (kStep) brings the raw projections: a warp normalises and rotates the query heads where it needs them, in the registers that
 // the products take; the block that has the pair's last tile does so for the key, writes key and value into the new row's place, in
@@ -36,6 +39,8 @@ constexpr int kTile = 64;                 // rows of a tile
 constexpr int kWarps = 4;                 // that compute; one more feeds them
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMostCluster = 8;           // blocks of a pair
+constexpr int kClusterTiles = 8;          // tiles of a block, up to which pairs have clusters
 
 __host__ __device__ constexpr int stage_bytes(int D) { return 2 * kTile * D * 2; }
 // floats of a lane that a warp hands over: its columns of each head it holds
@@ -50,11 +55,14 @@ __host__ __device__ constexpr int smem_bytes(int D, bool wide) {
   return 1024 + stages_of(D, wide) * stage_bytes(D) + merge_bytes(D, wide);
 }
 
-// What a pair is, for the second kernel.
-struct Pair {
-  int unit;               // its first tile in the line
-  int first, last;        // blocks that have tiles of it; first = -1: none
-  int rows;
+// For the second kernel: a block's stretch and the pairs at its ends.
+struct End {
+  int pair, unit;         // its first tile in the line
+  int first, last;        // blocks that have tiles of it
+};
+struct Stretch {
+  int blocks, begins, ends, pad;          // blocks that have one; this block's tiles
+  End end[2];
 };
 
 struct Args {
@@ -67,20 +75,26 @@ struct Args {
   int boxes, box_rows;    // pages of a tile, rows of a page that a tile takes
   bf16* out;
   int* status;
+  int cluster;            // blocks of a pair, or 0: stretches of the line
+  long long pair_tiles;   // that a pair has room for
   // workspace
-  int* units;             // [1]
-  int* block_pair;        // [blocks] the pair that a block begins with
-  Pair* pairs;            // [B hkv]
+  Stretch* stretches;     // [blocks of the grid]
   float* part;            // [blocks][2][G (D + 2)]: of the first pair of a block and of the last
-  int* unit_pair;         // [tiles]           where weights are asked for
-  float2* top_sum;        // [B hkv][G] maximum and sum of pairs that are not cut
+  int4* tile_rows;        // [tiles] pair, first row, rows of the sequence; this and the next two where weights are asked for
+  float2* top_sum;        // [B hkv][G] maximum and 1 / sum of pairs that are not cut
   float* scores;          // [tiles][G][64], times log2 e
 };
 
-__device__ __forceinline__ long long first_unit(long long units, int block, int blocks) { return units * block / blocks; }
-__device__ __forceinline__ int block_of(long long unit, long long units, int blocks) {
-  return static_cast<int>(((unit + 1) * blocks - 1) / units);
-}
+// Equal stretches of a line of `units` tiles: the first ones are a tile longer where it does not divide.
+struct Line {
+  unsigned each, longer;
+  __device__ __forceinline__ Line(unsigned units, unsigned blocks) : each(units / blocks), longer(units % blocks) {}
+  __device__ __forceinline__ int first(unsigned block) const { return block * each + min(block, longer); }
+  __device__ __forceinline__ int block_of(unsigned unit) const {
+    const unsigned head = longer * (each + 1);
+    return unit < head ? unit / (each + 1) : longer + (unit - head) / each;
+  }
+};
 
 // Rows of a sequence that this call attends to; -1 where table, length or position do not hold.
 template <bool kStep>
@@ -97,7 +111,7 @@ __device__ __forceinline__ int tiles_of(int rows) { return rows > 0 ? (rows + kT
 // A block's way along its stretch.
 struct Walk {
   int b, h, t, rows;
-  long long left;         // tiles of the stretch from here on
+  int left;               // tiles of the stretch from here on
 };
 template <bool kStep>
 __device__ __forceinline__ void next_pair(const Args& a, Walk& w, int taken) {
@@ -124,15 +138,31 @@ __device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::
 // l / 4 + 8 where there are more than eight). A head's columns j and j + D / 2 are in the same lane.
 template <int D, bool kStep>
 __device__ __forceinline__ void load_head(const Args& a, const bf16* x, bool there, int pos, int lane, float (&v)[D / 16][4]) {
+  constexpr int kAt = kStep ? D / 16 : 1;
   const int col = 2 * (lane & 3);
+  uint32_t two[D / 16][2], norm[kAt][2];
+  float2 cs[kAt][2], sn[kAt][2];
+  // everything is asked for at once
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int at = 16 * k + 8 * e + col;
+      two[k][e] = there ? *reinterpret_cast<const uint32_t*>(x + at) : 0u;
+      if constexpr (kStep) {
+        cs[k][e] = *reinterpret_cast<const float2*>(a.st.cos_t + static_cast<long long>(pos) * D + at);
+        sn[k][e] = *reinterpret_cast<const float2*>(a.st.sin_t + static_cast<long long>(pos) * D + at);
+        norm[k][e] = a.st.q_w ? *reinterpret_cast<const uint32_t*>(static_cast<const bf16*>(a.st.q_w) + at) : 0u;
+      }
+    }
+  }
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t two = there ? *reinterpret_cast<const uint32_t*>(x + 16 * k + 8 * e + col) : 0u;
-      v[k][2 * e] = bf_lo(two);
-      v[k][2 * e + 1] = bf_hi(two);
+      v[k][2 * e] = bf_lo(two[k][e]);
+      v[k][2 * e + 1] = bf_hi(two[k][e]);
       ss += v[k][2 * e] * v[k][2 * e] + v[k][2 * e + 1] * v[k][2 * e + 1];
     }
   }
@@ -145,20 +175,16 @@ __device__ __forceinline__ void load_head(const Args& a, const bf16* x, bool the
       for (int k = 0; k < D / 16; ++k) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t two = *reinterpret_cast<const uint32_t*>(static_cast<const bf16*>(a.st.q_w) + 16 * k + 8 * e + col);
-          v[k][2 * e] *= r * bf_lo(two);
-          v[k][2 * e + 1] *= r * bf_hi(two);
+          v[k][2 * e] *= r * bf_lo(norm[k][e]);
+          v[k][2 * e + 1] *= r * bf_hi(norm[k][e]);
         }
       }
     }
-    const float *cs = a.st.cos_t + static_cast<long long>(pos) * D + col, *sn = a.st.sin_t + static_cast<long long>(pos) * D + col;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int at = 16 * k + 8 * e;
-        const float2 c1 = *reinterpret_cast<const float2*>(cs + at), s1 = *reinterpret_cast<const float2*>(sn + at);
-        const float2 c2 = *reinterpret_cast<const float2*>(cs + at + D / 2), s2 = *reinterpret_cast<const float2*>(sn + at + D / 2);
+        const float2 c1 = cs[k][e], s1 = sn[k][e], c2 = cs[k + D / 32][e], s2 = sn[k + D / 32][e];
         float(&lo)[4] = v[k], (&hi)[4] = v[k + D / 32];
         const float x0 = lo[2 * e], x1 = lo[2 * e + 1], y0 = hi[2 * e], y1 = hi[2 * e + 1];
         lo[2 * e] = x0 * c1.x - y0 * s1.x;
@@ -198,7 +224,61 @@ __device__ __forceinline__ void new_key(const Args& a, const bf16* x, int pos, i
 // Byte of column x of row r within a tile: halves of 64 columns, rows of 128 bytes, 16-byte pieces exchanged by the row (as TMA does).
 __device__ __forceinline__ uint32_t place(int r, int x) { return (x >> 6) * (kTile * 128) + r * 128 + ((((x >> 3) & 7) ^ (r & 7)) << 4) + (x & 7) * 2; }
 
-template <int D, bool kWide, bool kStep>
+// Shares of the rows of tiles that this warp has scored, from the lanes that hold the scores: four rows of one or two heads each.
+template <int kHeads, bool kStep>
+__device__ __forceinline__ void add_weights(const Args& a, long long unit, int pair, int t0, int tiles, int rows, int warp, int lane,
+                                            const float2* final) {
+  const int g0 = lane >> 2, col = 16 * warp + 2 * (lane & 3);
+  float2 f[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) f[i] = final[g0 + 8 * i];
+  float* weights = a.c.weights + static_cast<long long>(pair) * a.c.width * a.c.page;
+  constexpr int kAhead = 4;                               // tiles whose loads are under way
+  for (int t1 = 0; t1 < tiles; t1 += kAhead) {
+    float2 x[kAhead][kHeads][2], old[kAhead];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      const long long at = unit + min(t1 + t, tiles - 1);
+      const int r = (t0 + t1 + t) * kTile + col + 8 * g0;             // of lanes that write: g0 = 0, 1
+      old[t] = g0 < 2 && t1 + t < tiles && r < rows ? *reinterpret_cast<const float2*>(weights + r) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const float* s = a.scores + (at * a.G + min(g0 + 8 * i, a.G - 1)) * kTile + col;
+        x[t][i][0] = *reinterpret_cast<const float2*>(s);
+        x[t][i][1] = *reinterpret_cast<const float2*>(s + 8);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      float2 p[2] = {};
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const float inv = g0 + 8 * i < a.G ? f[i].y : 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[e].x += inv == 0.f ? 0.f : exp2f(x[t][i][e].x - f[i].x) * inv;
+          p[e].y += inv == 0.f ? 0.f : exp2f(x[t][i][e].y - f[i].x) * inv;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          p[e].x += __shfl_xor_sync(0xffffffffu, p[e].x, o);
+          p[e].y += __shfl_xor_sync(0xffffffffu, p[e].y, o);
+        }
+      }
+      const int r = (t0 + t1 + t) * kTile + col + 8 * g0;
+      if (g0 < 2 && t1 + t < tiles && r < rows) {         // a new row's weight starts from 0
+        const float2 own = g0 ? p[1] : p[0];
+        weights[r] = (kStep && r == rows - 1 ? 0.f : old[t].x) + own.x;
+        if (r + 1 < rows) weights[r + 1] = (kStep && r + 1 == rows - 1 ? 0.f : old[t].y) + own.y;
+      }
+    }
+  }
+}
+
+template <int D, bool kWide, bool kStep, bool kCluster>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, kWide))
 paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
   constexpr int kStages = stages_of(D, kWide), kHalf = kTile * D * 2;
@@ -206,13 +286,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int kFloats = lane_floats(D, kWide);
   extern __shared__ unsigned char s_dyn[];
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
-  __shared__ long long s_scan[kThreads / 32];
+  __shared__ int s_scan[kThreads / 32];
   __shared__ Walk s_start;
+  __shared__ float2 s_final[16];                          // maximum and 1 / sum of a pair's heads
+  __shared__ float2 s_sums[16];                           // of this block (clusters)
   __shared__ int s_abort;
   unsigned char* ring = s_dyn + ((1024 - (smem_u32(s_dyn) & 1023)) & 1023);
   float* s_merge = reinterpret_cast<float*>(ring + kStages * stage_bytes(D));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int block = blockIdx.x, blocks = gridDim.x;
+  const int block = blockIdx.x;
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -227,58 +309,79 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   griddep_wait();
   griddep_launch_dependents();
 
-  // Tiles ahead of each sequence: every thread a run of sequences.
-  const int run = (a.B + kThreads - 1) / kThreads, from = min(a.B, tid * run), to = min(a.B, from + run);
-  long long mine = 0;
-  for (int b = from; b < to; ++b) {
-    const int rows = rows_of<kStep>(a, b);
-    mine += tiles_of(rows);
-    if (rows < 0 && block == 0) atomicMax(a.status, kStatusBounds);
-  }
-  long long before = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += up;
-  }
-  if (lane == 31) s_scan[warp] = before;
-  before -= mine;
-  __syncthreads();
-  long long units = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += s_scan[w];
-    units += s_scan[w];
-  }
-  units *= a.hkv;
-  before *= a.hkv;
-  mine *= a.hkv;
-  const long long u0 = first_unit(units, block, blocks), u1 = first_unit(units, block + 1, blocks);
-  if (u1 > u0 && u0 >= before && u0 < before + mine) {
-    long long at = before;
-    int b = from, rows = 0;
-    for (;; ++b) {
-      rows = rows_of<kStep>(a, b);
-      const long long all = static_cast<long long>(tiles_of(rows)) * a.hkv;
-      if (u0 < at + all) break;
-      at += all;
+  long long unit = 0;                                     // of scores
+  int units = 0, blocks = 0;                              // of the line; that have a stretch
+  Walk w;
+  if constexpr (kCluster) {
+    const int pair = block / a.cluster, rank = block - pair * a.cluster, b = pair / a.hkv;
+    const int rows = rows_of<kStep>(a, b), tiles = tiles_of(rows);
+    if (rows <= 0) {                                      // all blocks of the pair
+      if (rows < 0 && tid == 0) atomicMax(a.status, kStatusBounds);
+      if (rank == 0 && tid < a.G * D / 8)
+        for (int i = tid; i < a.G * D / 8; i += kThreads)
+          reinterpret_cast<uint4*>(a.out + static_cast<long long>(pair) * a.G * D)[i] = make_uint4(0, 0, 0, 0);
+      return;
     }
-    const int tiles = tiles_of(rows), h = static_cast<int>((u0 - at) / tiles);
-    s_start = {b, h, static_cast<int>(u0 - at - static_cast<long long>(h) * tiles), rows, u1 - u0};
-    a.block_pair[block] = b * a.hkv + h;
+    const int t0 = rank * tiles / a.cluster;
+    w = {b, pair - b * a.hkv, t0, rows, (rank + 1) * tiles / a.cluster - t0};
+    unit = pair * a.pair_tiles + t0;
+    __syncthreads();
+  } else {
+    // Tiles ahead of each sequence: every thread a run of sequences.
+    const int run = (a.B + kThreads - 1) / kThreads, from = min(a.B, tid * run), to = min(a.B, from + run);
+    int mine = 0;
+    for (int b = from; b < to; ++b) {
+      const int rows = rows_of<kStep>(a, b);
+      mine += tiles_of(rows);
+      if (rows < 0 && block == 0) atomicMax(a.status, kStatusBounds);
+    }
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    if (lane == 31) s_scan[warp] = before;
+    before -= mine;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kThreads / 32; ++x) {
+      if (x < warp) before += s_scan[x];
+      units += s_scan[x];
+    }
+    units *= a.hkv;
+    before *= a.hkv;
+    mine *= a.hkv;
+    blocks = min(static_cast<int>(gridDim.x), units);
+    if (block < blocks) {
+      const Line line(units, blocks);
+      const int u0 = line.first(block), u1 = line.first(block + 1);
+      if (u0 >= before && u0 < before + mine) {
+        int at = before, b = from, rows = 0;
+        for (;; ++b) {
+          rows = rows_of<kStep>(a, b);
+          const int all = tiles_of(rows) * a.hkv;
+          if (u0 < at + all) break;
+          at += all;
+        }
+        const int tiles = tiles_of(rows), h = (u0 - at) / tiles;
+        s_start = {b, h, u0 - at - h * tiles, rows, u1 - u0};
+      }
+      unit = u0;
+    }
+    // sequences without rows: zeros
+    for (int b = block; b < a.B; b += gridDim.x) {
+      if (rows_of<kStep>(a, b) > 0) continue;
+      for (int i = tid; i < a.hkv * a.G * D / 8; i += kThreads)
+        reinterpret_cast<uint4*>(a.out + static_cast<long long>(b) * a.hkv * a.G * D)[i] = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    if (tid == 0) a.stretches[block].blocks = blocks;
+    if (block >= blocks) return;
+    w = s_start;
+    if (tid == 0) a.stretches[block].begins = static_cast<int>(unit), a.stretches[block].ends = static_cast<int>(unit) + w.left;
   }
-  if (tid == 0 && block == 0) *a.units = static_cast<int>(units);
-  // sequences without rows: zeros
-  for (int b = block; b < a.B; b += blocks) {
-    if (rows_of<kStep>(a, b) > 0) continue;
-    for (int i = tid; i < a.hkv * a.G * D / 8; i += kThreads)
-      reinterpret_cast<uint4*>(a.out + static_cast<long long>(b) * a.hkv * a.G * D)[i] = make_uint4(0, 0, 0, 0);
-    for (int h = tid; h < a.hkv; h += kThreads) a.pairs[b * a.hkv + h] = {0, -1, -1, 0};
-  }
-  __syncthreads();
-  if (u1 <= u0) return;
 
-  Walk w = s_start;
   int stage = 0, phase = 0;
   auto advance = [&] {
     if (++stage == kStages) {
@@ -294,7 +397,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const bool value = part >= D / 64;
     const int x = part % (D / 64) * 64;
     while (w.left > 0) {
-      const int tiles = tiles_of(w.rows), take = static_cast<int>(min(static_cast<long long>(tiles - w.t), w.left));
+      const int tiles = tiles_of(w.rows), take = min(tiles - w.t, w.left);
       const int* table = a.c.table + w.b * a.c.table_stride;
       for (int t = w.t; t < w.t + take; ++t) {
         const int row = t * kTile + box * a.box_rows;
@@ -318,18 +421,18 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       next_pair<kStep>(a, w, take);
     }
-    return;
+    if (!kCluster) return;
   }
 
   // ---------------------------------------------------------------------- computes
   const int g0 = lane >> 2, col = 2 * (lane & 3);
-  long long unit = u0;
+  const long long unit0 = unit;
   bool handed = false;                                    // the buffers of the warps' sums are in use
   bool first_pair = true;
-  while (w.left > 0) {
-    const int tiles = tiles_of(w.rows), take = static_cast<int>(min(static_cast<long long>(tiles - w.t), w.left));
+  while (warp < kWarps && (kCluster || w.left > 0)) {
+    const int tiles = tiles_of(w.rows), take = min(tiles - w.t, w.left);
     const int pair = w.b * a.hkv + w.h;
-    const bool last_tile = w.t + take == tiles;
+    const bool last_tile = w.t + take == tiles && take > 0;
     int pos = 0;
     if constexpr (kStep) pos = a.st.positions[w.b];
     const bf16* q = a.q + w.b * a.q_stride;
@@ -382,8 +485,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         static_cast<bf16*>(a.c.v)[at + lane + 32 * i] = nv[i];
       }
     }
-    if (w.t == 0 && tid == 0)
-      a.pairs[pair] = {static_cast<int>(unit), block, block_of(unit + tiles - 1, first_unit(units, blocks, blocks), blocks), w.rows};
+    if (!kCluster && tid == 0 && (first_pair || take == w.left)) {
+      const Line line(units, blocks);
+      const int at = static_cast<int>(unit) - w.t;
+      const End end = {pair, at, line.block_of(at), line.block_of(at + tiles - 1)};
+      if (first_pair) a.stretches[block].end[0] = end;
+      if (take == w.left) a.stretches[block].end[1] = end;
+    }
 
     float m[kHeads], l[kHeads], o[D / 8][4];
 #pragma unroll
@@ -398,7 +506,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       if (!mbar_wait(&s_full[stage], phase, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
       const uint32_t ks = smem_u32(ring + stage * stage_bytes(D)), vs = ks + kHalf;
       const int r0 = 16 * warp, valid = w.rows - t * kTile - r0;   // of this warp's 16 rows
-      if (a.unit_pair && tid == 0) a.unit_pair[unit] = pair;
+      if (!kCluster && a.scores && tid == 0) a.tile_rows[unit] = make_int4(pair, t * kTile, w.rows, 0);
       if (valid > 0) {
         if (kStep && owner && t == tiles - 1) {
 #pragma unroll
@@ -557,18 +665,28 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           f[4 * x + 3] = f[4 * x + 3] * own[kHeads - 1] + v.w * its[kHeads - 1];
         }
       }
+      const bool whole = w.t == 0 && last_tile;
+      if constexpr (kCluster) {
+        // for the other blocks: where the second warp's sums have been, and the heads' maxima and sums
+        float4* to_others = reinterpret_cast<float4*>(s_merge);
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i) {
-        const int g = g0 + 8 * i;
-        if (g < a.G) {
-          if (w.t == 0 && last_tile) {                    // the whole pair
+        for (int x = 0; x < kFloats / 4; ++x) to_others[x * 32 + lane] = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i)
+          if ((lane & 3) == 0) s_sums[g0 + 8 * i] = make_float2(m[i], l[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          const int g = g0 + 8 * i;
+          if (g >= a.G) continue;
+          if (whole) {
             const float inv = 1.f / l[i];
             bf16* out = a.out + (static_cast<long long>(pair) * a.G + g) * D + col;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j)
               *reinterpret_cast<uint32_t*>(out + 8 * j) =
                   bf_pack(f[2 * kHeads * j + 2 * i] * inv, f[2 * kHeads * j + 2 * i + 1] * inv);
-            if (a.top_sum && (lane & 3) == 0) a.top_sum[pair * a.G + g] = make_float2(m[i], l[i]);
+            if (a.scores && (lane & 3) == 0) a.top_sum[pair * a.G + g] = make_float2(m[i], inv);
           } else {
             float* part = a.part + (2LL * block + (first_pair ? 0 : 1)) * a.G * (D + 2);
 #pragma unroll
@@ -583,87 +701,136 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         }
       }
     }
+    if constexpr (kCluster) break;
     first_pair = false;
     next_pair<kStep>(a, w, take);
   }
+  if constexpr (kCluster) {
+    // Every block adds the heads' maxima and sums, the first one the columns too: a warp a share of them.
+    __syncwarp();
+    cluster_sync_all();
+    const int pair = block / a.cluster, rank = block - pair * a.cluster;
+    if (tid < 16) {
+      float top = -FLT_MAX, sum = 0.f;
+      for (int c = 0; c < a.cluster; ++c) {
+        const uint32_t at = map_to_cta(smem_u32(&s_sums[tid]), c);
+        float2 ml;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(at) : "memory");
+        const float next = fmaxf(top, ml.x);
+        sum = sum * exp2f(top - next) + ml.y * exp2f(ml.x - next);
+        top = next;
+      }
+      s_final[tid] = make_float2(top, 1.f / sum);
+    }
+    __syncthreads();
+    if (rank == 0 && warp < kWarps) {
+#pragma unroll
+      for (int x0 = 0; x0 < kFloats / 4; x0 += kWarps) {
+        const int x = x0 + warp;                          // columns 16 x .. of a head, or 8 x .. of the lane's two
+        if (x >= kFloats / 4) continue;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int ga = g0, gb = kWide ? g0 + 8 : g0;
+        const float2 fa = s_final[ga], fb = s_final[gb];
+        for (int c = 0; c < a.cluster; ++c) {
+          const float4 p = ld_shared_cluster_f4(map_to_cta(smem_u32(s_merge) + (x * 32 + lane) * 16, c));
+          float ma, mb;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ma) : "r"(map_to_cta(smem_u32(&s_sums[ga]), c)) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(mb) : "r"(map_to_cta(smem_u32(&s_sums[gb]), c)) : "memory");
+          const float ea = exp2f(ma - fa.x), eb = exp2f(mb - fb.x);
+          v.x += p.x * ea;
+          v.y += p.y * ea;
+          v.z += p.z * eb;
+          v.w += p.w * eb;
+        }
+        bf16* out = a.out + static_cast<long long>(pair) * a.G * D;
+        const int first = kWide ? 8 * x : 16 * x, second = kWide ? 8 * x : 16 * x + 8;
+        if (ga < a.G) *reinterpret_cast<uint32_t*>(out + ga * D + first + col) = bf_pack(v.x * fa.y, v.y * fa.y);
+        if (gb < a.G) *reinterpret_cast<uint32_t*>(out + gb * D + second + col) = bf_pack(v.z * fb.y, v.w * fb.y);
+      }
+    }
+    if (a.scores && warp < kWarps) add_weights<kHeads, kStep>(a, unit0, pair, w.t, w.left, w.rows, warp, lane, s_final);
+    __syncwarp();
+    cluster_sync_all();                                   // nobody leaves while its sums are being read
+  }
 }
 
-// The sums of block `c`'s part of a pair.
-__device__ __forceinline__ const float* part_of(const Args& a, const Pair& p, int c, long long units, int blocks, int D) {
-  const bool starts = first_unit(units, c, blocks) >= p.unit;     // the block begins with this pair
-  return a.part + (2LL * c + (starts ? 0 : 1)) * a.G * (D + 2);
-}
 
+constexpr int kMostBlocks = 2 * 160;
 constexpr int kFinishThreads = 256;
 
-// Pairs that several blocks share: block c those whose first cut is the start of stretch c. Then the weights, a warp a tile.
+// What a stretch has left: the pairs at its two ends where they are cut (their output, by the block behind the first cut), half of
+// the warps each; then the weights of its tiles, a warp a tile.
 template <bool kStep>
-__global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args a, int blocks, int D) {
+__global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args a, int D) {
+  constexpr int kHalf = kFinishThreads / 2;
+  __shared__ float s_scale[2][kMostBlocks * 16];          // of a part's head
+  __shared__ float2 s_final[2][16];
   griddep_wait();
   griddep_launch_dependents();
-  const long long units = *a.units;
-  const int tid = threadIdx.x, G = a.G;
-  if (units == 0) return;
-  if (blockIdx.x > 0 && static_cast<int>(blockIdx.x) < blocks) {
-    const int c = blockIdx.x;
-    const long long u = first_unit(units, c, blocks);
-    if (u < first_unit(units, c + 1, blocks)) {
-      const int pair = a.block_pair[c];
-      const Pair p = a.pairs[pair];
-      // the stretches ahead that are empty begin at the same tile
-      if (p.unit < u && p.first < c && block_of(u - 1, units, blocks) == p.first) {
-        for (int i = tid; i < G * D; i += kFinishThreads) {
-          const int g = i / D;
-          float m = -FLT_MAX, l = 0.f, v = 0.f;
-          for (int x = p.first; x <= p.last; ++x) {
-            if (first_unit(units, x, blocks) == first_unit(units, x + 1, blocks)) continue;
-            const float* part = part_of(a, p, x, units, blocks, D);
-            const float pm = part[G * D + 2 * g], top = fmaxf(m, pm), f = exp2f(m - top), e = exp2f(pm - top);
-            v = v * f + part[i] * e;
-            l = l * f + part[G * D + 2 * g + 1] * e;
-            m = top;
-          }
-          a.out[static_cast<long long>(pair) * G * D + i] = from_f32<bf16>(v / l);
-        }
+  const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.G;
+  const Stretch st = a.stretches[c];
+  if (c >= st.blocks) return;
+  // the warp's first tile is asked for ahead of everything
+  int u = st.begins + warp;
+  const bool tile = a.scores && u < st.ends;
+  int4 at = tile ? a.tile_rows[u] : make_int4(-1, 0, 0, 0);
+
+  const int half = tid >= kHalf, in_half = tid - half * kHalf;
+  const End p = half ? st.end[1] : st.end[0];
+  const bool cut = p.first < p.last && !(half && st.end[0].pair == p.pair);
+  const int parts = p.last - p.first + 1;
+  // the first block may have begun with another pair
+  const float* first = a.part + (2LL * p.first + (p.first == c ? (half && st.begins < p.unit) : a.stretches[p.first].begins < p.unit)) * G * (D + 2);
+  auto part = [&](int x) { return x == 0 ? first : a.part + 2LL * (p.first + x) * G * (D + 2); };
+  if (cut) {
+    for (int g = in_half >> 5; g < G; g += kHalf / 32) {
+      float top = -FLT_MAX, sum = 0.f;
+      for (int x = lane; x < parts; x += 32) top = fmaxf(top, part(x)[G * D + 2 * g]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int x = lane; x < parts; x += 32) {
+        const float2 ml = *reinterpret_cast<const float2*>(part(x) + G * D + 2 * g);
+        const float f = exp2f(ml.x - top);
+        s_scale[half][x * G + g] = f;
+        sum += ml.y * f;
       }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s_final[half][g] = make_float2(top, 1.f / sum);
+    }
+  }
+  __syncthreads();
+  if (cut && c == p.first + 1) {
+    for (int i = in_half; i < G * D; i += kHalf) {
+      const int g = i / D;
+      float v = 0.f;
+#pragma unroll 8
+      for (int x = 0; x < parts; ++x) v += part(x)[i] * s_scale[half][x * G + g];
+      a.out[static_cast<long long>(p.pair) * G * D + i] = from_f32<bf16>(v * s_final[half][g].y);
     }
   }
   if (!a.scores) return;
-  const int lane = tid & 31;
-  const long long limit = static_cast<long long>(a.c.width) * a.c.page;
-  for (long long u = blockIdx.x * (kFinishThreads / 32LL) + (tid >> 5); u < units; u += gridDim.x * (kFinishThreads / 32LL)) {
-    const int pair = a.unit_pair[u];
-    const Pair p = a.pairs[pair];
-    float top = 0.f, inv = 0.f;                           // lane g: of head g
-    if (lane < G) {
-      float m = -FLT_MAX, l = 0.f;
-      if (p.first == p.last) {
-        const float2 ml = a.top_sum[pair * G + lane];
-        m = ml.x;
-        l = ml.y;
-      } else {
-        for (int x = p.first; x <= p.last; ++x) {
-          if (first_unit(units, x, blocks) == first_unit(units, x + 1, blocks)) continue;
-          const float* part = part_of(a, p, x, units, blocks, D) + G * D + 2 * lane;
-          const float next = fmaxf(m, part[0]);
-          l = l * exp2f(m - next) + part[1] * exp2f(part[0] - next);
-          m = next;
-        }
-      }
-      top = m;
-      inv = 1.f / l;
+  for (; u < st.ends; u += kFinishThreads / 32) {
+    const int row = at.y + 2 * lane, rows = at.z;
+    float* w = a.c.weights + static_cast<long long>(at.x) * a.c.width * a.c.page + row;
+    const float2 old = row < rows ? *reinterpret_cast<const float2*>(w) : make_float2(0.f, 0.f);
+    const float2* final = a.top_sum + static_cast<long long>(at.x) * G;
+    if (at.x == st.end[0].pair && st.end[0].first < st.end[0].last) {
+      final = s_final[0];
+    } else if (at.x == st.end[1].pair && st.end[1].first < st.end[1].last) {
+      final = s_final[1];
     }
-    const int row = static_cast<int>(u - p.unit) * kTile + 2 * lane;
     float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
     for (int g = 0; g < G; ++g) {
-      const float2 s = *reinterpret_cast<const float2*>(a.scores + (u * G + g) * kTile + 2 * lane);
-      const float tg = __shfl_sync(0xffffffffu, top, g), ig = __shfl_sync(0xffffffffu, inv, g);
-      s0 += exp2f(s.x - tg) * ig;
-      s1 += exp2f(s.y - tg) * ig;
+      const float2 s = *reinterpret_cast<const float2*>(a.scores + (static_cast<long long>(u) * G + g) * kTile + 2 * lane), f = final[g];
+      s0 += exp2f(s.x - f.x) * f.y;
+      s1 += exp2f(s.y - f.x) * f.y;
     }
-    float* w = a.c.weights + pair * limit + row;
-    if (row < p.rows) w[0] = (kStep && row == p.rows - 1 ? 0.f : w[0]) + s0;
-    if (row + 1 < p.rows) w[1] = (kStep && row + 1 == p.rows - 1 ? 0.f : w[1]) + s1;
+    // a new row's weight starts from 0
+    if (row < rows) w[0] = (kStep && row == rows - 1 ? 0.f : old.x) + s0;
+    if (row + 1 < rows) w[1] = (kStep && row + 1 == rows - 1 ? 0.f : old.y) + s1;
+    if (u + kFinishThreads / 32 < st.ends) at = a.tile_rows[u + kFinishThreads / 32];
   }
 }
 
@@ -673,12 +840,18 @@ int sm_count() {
   return n;
 }
 
-// Where things lie in the workspace; blocks is what the launch has at most, whatever the device.
+// Blocks of a pair where short caches take clusters, else 0.
+int cluster_of(long long pairs, long long tiles) {
+  int blocks = 1;
+  while (blocks < kMostCluster && 2 * blocks * pairs <= 2LL * sm_count() && 2 * blocks <= tiles) blocks *= 2;
+  return blocks * pairs <= 2LL * sm_count() && (tiles + blocks - 1) / blocks <= kClusterTiles ? blocks : 0;
+}
+
+// Where things lie in the workspace.
 struct Layout {
-  long long tiles;
-  size_t block_pair, pairs, part, unit_pair, top_sum, scores, bytes;
+  long long tiles;        // of a pair
+  size_t part, tile_rows, top_sum, scores, bytes;
 };
-constexpr int kMostBlocks = 2 * 160;
 Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
   Layout l = {};
   auto take = [&](size_t n) {
@@ -687,27 +860,45 @@ Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
     return at;
   };
   const long long rows = static_cast<long long>(width) * page, pairs = static_cast<long long>(B) * hkv;
-  l.tiles = pairs * ((rows + kTile - 1) / kTile);
-  l.bytes = 256;                                          // units
-  l.block_pair = take(sizeof(int) * kMostBlocks);
-  l.pairs = take(sizeof(Pair) * pairs);
+  l.tiles = (rows + kTile - 1) / kTile;
+  take(sizeof(Stretch) * kMostBlocks);
   l.part = take(sizeof(float) * kMostBlocks * 2 * G * (D + 2));
-  l.unit_pair = weights ? take(sizeof(int) * l.tiles) : 0;
+  l.tile_rows = weights ? take(sizeof(int4) * l.tiles * pairs) : 0;
   l.top_sum = weights ? take(sizeof(float2) * pairs * G) : 0;
-  l.scores = weights ? take(sizeof(float) * l.tiles * G * kTile) : 0;
+  l.scores = weights ? take(sizeof(float) * l.tiles * pairs * G * kTile) : 0;
   return l;
 }
 
 template <int D, bool kWide, bool kStep>
-cudaError_t launch_one(const CUtensorMap& k, const CUtensorMap& v, const Args& a, long long tiles, cudaStream_t stream) {
-  constexpr auto kKernel = paged_attention_kernel<D, kWide, kStep>;
+cudaError_t launch_one(const CUtensorMap& k, const CUtensorMap& v, const Args& a, cudaStream_t stream) {
+  const long long pairs = static_cast<long long>(a.B) * a.hkv;
+  if (a.cluster) {
+    constexpr auto kKernel = paged_attention_kernel<D, kWide, kStep, true>;
+    const cudaError_t e = allow_smem<kKernel>(smem_bytes(D, kWide));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(pairs * a.cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem_bytes(D, kWide);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kKernel, k, v, a);
+  }
+  constexpr auto kKernel = paged_attention_kernel<D, kWide, kStep, false>;
   cudaError_t e = allow_smem<kKernel>(smem_bytes(D, kWide));
   if (e != cudaSuccess) return e;
   const long long most = sm_count() * blocks_per_sm(D, kWide) < kMostBlocks ? sm_count() * blocks_per_sm(D, kWide) : kMostBlocks;
-  const int blocks = static_cast<int>(tiles < most ? tiles : most);
+  const int blocks = static_cast<int>(pairs * a.pair_tiles < most ? pairs * a.pair_tiles : most);
   e = launch_kernel(kKernel, dim3(blocks), dim3(kThreads), smem_bytes(D, kWide), stream, k, v, a);
   if (e != cudaSuccess) return e;
-  return launch_kernel(paged_finish_kernel<kStep>, dim3(a.scores && blocks > 8 ? 2 * blocks : blocks), dim3(kFinishThreads), 0, stream, a, blocks, D);
+  return launch_kernel(paged_finish_kernel<kStep>, dim3(blocks), dim3(kFinishThreads), 0, stream, a, D);
 }
 
 }  // namespace
@@ -733,12 +924,12 @@ cudaError_t launch_paged_attention(const cd_paged& c, const cd_paged_step* step,
   a.boxes = kTile / a.box_rows;
   a.out = static_cast<bf16*>(out);
   a.status = status;
-  a.units = reinterpret_cast<int*>(base);
-  a.block_pair = reinterpret_cast<int*>(base + l.block_pair);
-  a.pairs = reinterpret_cast<Pair*>(base + l.pairs);
+  a.pair_tiles = l.tiles;
+  a.cluster = cluster_of(static_cast<long long>(B) * hkv, l.tiles);
+  a.stretches = reinterpret_cast<Stretch*>(base);
   a.part = reinterpret_cast<float*>(base + l.part);
-  a.unit_pair = c.weights ? reinterpret_cast<int*>(base + l.unit_pair) : nullptr;
-  a.top_sum = c.weights ? reinterpret_cast<float2*>(base + l.top_sum) : nullptr;
+  a.tile_rows = reinterpret_cast<int4*>(base + l.tile_rows);
+  a.top_sum = reinterpret_cast<float2*>(base + l.top_sum);
   a.scores = c.weights ? reinterpret_cast<float*>(base + l.scores) : nullptr;
   CUtensorMap k, v;
   const int dims[4] = {D, c.page, hkv, c.pages};
@@ -747,7 +938,7 @@ cudaError_t launch_paged_attention(const cd_paged& c, const cd_paged_step* step,
     return cudaErrorInvalidValue;
 #define CDEEP_PAGED(DD, WIDE)                                                                                     \
   if (D == DD && (a.G > 8) == WIDE)                                                                               \
-    return step ? launch_one<DD, WIDE, true>(k, v, a, l.tiles, stream) : launch_one<DD, WIDE, false>(k, v, a, l.tiles, stream);
+    return step ? launch_one<DD, WIDE, true>(k, v, a, stream) : launch_one<DD, WIDE, false>(k, v, a, stream);
   CDEEP_PAGED(64, false) CDEEP_PAGED(64, true) CDEEP_PAGED(128, false) CDEEP_PAGED(128, true)
 #undef CDEEP_PAGED
   return cudaErrorInvalidValue;

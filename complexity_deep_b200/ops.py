@@ -1395,59 +1395,74 @@ def combine_top_(stream: torch.Tensor, y: torch.Tensor, inv_perm: torch.Tensor, 
 
 
 # --------------------------------------------------------------------------- paged cache
-def _on(t: torch.Tensor, name: str, dtype, device, shape) -> int:
-    """Address of a contiguous tensor of that type, device and shape."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or tuple(t.shape) != shape:
-        raise RuntimeError(f"{name}: expected a {dtype} tensor of shape {list(shape)} on {device}")
-    if not t.is_contiguous():
-        raise RuntimeError(f"{name}: expected a contiguous tensor")
-    return t.data_ptr()
+def _on(t: torch.Tensor, name: str, dtype, device: int, shape) -> int:
+    """Address of a contiguous CUDA tensor of that type, device index and shape."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda
+            and t.get_device() == device):
+        return t.data_ptr()
+    raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {list(shape)} on cuda:{device}")
 
 
-def _here(t: torch.Tensor, name: str):
-    """Device of a CUDA tensor, which has to be the current one: launches go to its current stream."""
+def _here(t: torch.Tensor, name: str) -> int:
+    """Device index of a CUDA tensor, which has to be the current one: launches go to its current stream."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name}: expected a CUDA tensor; the complexity_deep_b200 kernels have no CPU path")
-    if t.device.index != _current_device():
+    device = t.get_device()
+    if device != _current_device():
         raise RuntimeError(f"{name} is on {t.device}, the current device is cuda:{_current_device()}")
-    return t.device
+    return device
 
 
 def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
-           weights: Optional[torch.Tensor], layers: int, batch: int, device) -> _lib.Paged:
+           weights: Optional[torch.Tensor], layers: int, batch: int, device: int) -> _lib.Paged:
     """The cache as the library takes it; pools [pages, kv heads, page, D], of several layers with the layers in front."""
     shape, strides = k_pages.shape, k_pages.stride()
-    for t, name in ((k_pages, "k pages"), (v_pages, "v pages")):
-        if t.dtype is not BF16 or t.device != device or t.dim() < 4 or t.stride(-1) != 1:
-            raise RuntimeError(f"{name}: expected bf16 [pages, kv heads, page, D] on {device}, D contiguous")
-    if v_pages.shape != shape or v_pages.stride() != strides:
-        raise RuntimeError("k and v pages must share their shape and strides")
-    if any(n % 8 for n in strides[:-1]) or (k_pages.data_ptr() | v_pages.data_ptr()) & 15:
-        raise RuntimeError("pages: strides must be multiples of 8 elements, the pools lie on 16-byte boundaries")
-    if (block_table.dtype is not torch.int32 or block_table.device != device or block_table.dim() != 2
-            or block_table.shape[0] != batch or block_table.shape[1] < 1 or block_table.stride(1) != 1):
-        raise RuntimeError(f"block_table: expected int32 [{batch}, pages of a sequence] on {device}")
     pages, hkv, page, _ = shape[-4:]
+    stride_p, stride_h, stride_t, stride_d = strides[-4:]
+    k, v = k_pages.data_ptr(), v_pages.data_ptr()
+    if (k_pages.dtype is not BF16 or v_pages.dtype is not BF16 or stride_d != 1 or v_pages.shape != shape
+            or v_pages.stride() != strides or not (k_pages.is_cuda and v_pages.is_cuda)
+            or not k_pages.get_device() == device == v_pages.get_device()):
+        raise RuntimeError(f"pages: expected bf16 [pages, kv heads, page, D] on cuda:{device}, D contiguous, keys and values with the "
+                           "same shape and strides")
+    if (stride_p | stride_h | stride_t | strides[0]) & 7 or (k | v) & 15:
+        raise RuntimeError("pages: strides must be multiples of 8 elements, the pools lie on 16-byte boundaries")
+    if (block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] < 1
+            or block_table.stride(1) != 1 or not block_table.is_cuda or block_table.get_device() != device):
+        raise RuntimeError(f"block_table: expected int32 [{batch}, pages of a sequence] on cuda:{device}")
     width = block_table.shape[1]
-    statistics = (layers, batch, hkv, width * page) if len(shape) == 5 else (batch, hkv, width * page)
-    return _lib.Paged(k_pages.data_ptr(), v_pages.data_ptr(), strides[-4], strides[-3], strides[-2], block_table.data_ptr(),
-                      block_table.stride(0), _on(lengths, "lengths", torch.int32, device, (batch,)),
-                      None if weights is None else _on(weights, "weights", torch.float32, device, statistics), pages, page, width)
+    w = None
+    if weights is not None:
+        w = _on(weights, "weights", torch.float32, device,
+                (layers, batch, hkv, width * page) if len(shape) == 5 else (batch, hkv, width * page))
+    return _lib.Paged(k, v, stride_p, stride_h, stride_t, block_table.data_ptr(), block_table.stride(0),
+                      _on(lengths, "lengths", torch.int32, device, (batch,)), w, pages, page, width)
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(*sizes) -> int:
+    return _lib.load().cd_paged_attention_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _evict_workspace(*sizes) -> int:
+    return _lib.load().cd_evict_rows_workspace_bytes(*sizes)
 
 
 def _attend_paged(step, c: _lib.Paged, q: torch.Tensor, hq: int, hkv: int, D: int) -> torch.Tensor:
     lib = _lib.load()
-    B, device = q.shape[0], q.device
-    out = torch.empty(B, hq * D, dtype=BF16, device=device)
-    n = lib.cd_paged_attention_workspace_bytes(B, hq, hkv, D, c.page, c.width, 0 if c.weights is None else 1)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    with _Span("paged_attention"):
+    B = q.shape[0]
+    out = q.new_empty(B, hq * D)
+    n = _paged_workspace(B, hq, hkv, D, c.page, c.width, 0 if c.weights is None else 1)
+    ws = q.new_empty(n // 2)
+    with _Span("paged_attention", 2):
         if step is None:
-            _lib.check(lib.cd_paged_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), D ** -0.5, B, hq, hkv, D, out.data_ptr(),
-                                              _ptr(ws), n, _stream()), "cd_paged_attention")
+            status = lib.cd_paged_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), D ** -0.5, B, hq, hkv, D, out.data_ptr(),
+                                            ws.data_ptr(), n, _stream())
         else:
-            _lib.check(lib.cd_paged_step_attention(ctypes.byref(c), ctypes.byref(step), q.data_ptr(), D ** -0.5, B, hq, hkv, D,
-                                                   out.data_ptr(), _ptr(ws), n, _stream()), "cd_paged_step_attention")
+            status = lib.cd_paged_step_attention(ctypes.byref(c), ctypes.byref(step), q.data_ptr(), D ** -0.5, B, hq, hkv, D,
+                                                 out.data_ptr(), ws.data_ptr(), n, _stream())
+    _lib.check(status, "cd_paged_attention" if step is None else "cd_paged_step_attention")
     return out
 
 
@@ -1535,7 +1550,7 @@ def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
         raise RuntimeError("evict_rows_: both outputs or none")
     B = block_table.shape[0]
     c = _paged(k_pages, v_pages, block_table, lengths, weights, layers, B, device)
-    shape = tuple(weights.shape)
+    shape = weights.shape
     if weights_out is None:
         weights_out, row_positions_out = weights, row_positions
     e = _lib.Evict(_on(positions, "positions", torch.int32, device, (B,)),
@@ -1543,8 +1558,8 @@ def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
                    _on(weights_out, "weights_out", torch.float32, device, shape),
                    _on(row_positions_out, "row_positions_out", torch.int32, device, shape), keep, recent)
     lib = _lib.load()
-    n = lib.cd_evict_rows_workspace_bytes(layers, B, hkv, c.page, c.width, keep)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    n = _evict_workspace(layers, B, hkv, c.page, c.width, keep)
+    ws = k_pages.new_empty(n // 2) if n else None
     with _Span("evict_rows"):
         _lib.check(lib.cd_evict_rows(ctypes.byref(c), ctypes.byref(e), layers, k_pages.stride(0) if k_pages.dim() == 5 else 0, B, hkv, D,
                                      _ptr(ws), n, _stream()), "cd_evict_rows")
@@ -1573,8 +1588,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
             setattr(r, name + "s", _on(rule, name, dtype, device, (B,)))
         else:
             setattr(r, name, rule)
-    ids = torch.empty(B, dtype=torch.int64, device=device)
-    probs = torch.empty(B, dtype=torch.float32, device=device)
+    ids, probs = uniform.new_empty(B, dtype=torch.int64), uniform.new_empty(B)
     if B:
         with _Span("sample_tokens"):
             _lib.check(_lib.load().cd_sample_tokens(logits.data_ptr(), int(logits.dtype is torch.float32), logits.stride(0), B, V,
