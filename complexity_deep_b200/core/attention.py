@@ -27,6 +27,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ._cache import DerivedCache
+from .paged import PagedKVLayer
 from .rotary import RotaryEmbedding
 
 
@@ -202,6 +203,9 @@ class ComplexityAttention(nn.Module):
         if isinstance(past_key_value, StaticKVLayer):
             return (self._attend_static(x2, mu2, past_key_value, S, attention_mask),
                     past_key_value if use_cache else None)
+        if isinstance(past_key_value, PagedKVLayer):
+            return (self._attend_paged(x2, mu2, past_key_value, S, attention_mask),
+                    past_key_value if use_cache else None)
         past_len = past_key_value[0].shape[2] if past_key_value is not None else 0
         cos, sin = self.rotary_emb.tables_fp32(past_len + S)
         qkv = ops.mu_qkv_rope(x2, mu2, self._w_qkv(), self._w_mu() if mu2 is not None else None,
@@ -263,6 +267,16 @@ class ComplexityAttention(nn.Module):
         return ops.decode_step_attention(qkv, self.q_norm.weight if self.use_qk_norm else None,
                                          self.k_norm.weight if self.use_qk_norm else None, cos, sin, 1e-6,
                                          hq, hkv, D, past.k, past.v, cache.state[0:1], cache.state[1:2])
+
+    def _attend_paged(self, x2, mu2, past: PagedKVLayer, S, attention_mask) -> torch.Tensor:
+        """Decode step on a PagedKVCache: projection, then norm, rotation, append and attention at every slot's own position."""
+        hq, hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
+        if S != 1 or attention_mask is not None or x2.shape[0] != past.cache.slots:
+            raise RuntimeError("a PagedKVCache takes one new token per slot and no mask (steps attend to all of a sequence's rows)")
+        cos, sin = self.rotary_emb.tables_fp32(past.cache.max_positions)
+        qkv = ops.mu_qkv(x2, mu2, self._w_qkv(), self._w_mu() if mu2 is not None else None)
+        return past.step(qkv, self.q_norm.weight if self.use_qk_norm else None, self.k_norm.weight if self.use_qk_norm else None,
+                         cos, sin, 1e-6, hq, hkv, D)
 
     def _prefill_kernel_applies(self, B, S, attention_mask, past_key_value) -> bool:
         if attention_mask is not None or past_key_value is not None or not _PREFILL_KERNEL:

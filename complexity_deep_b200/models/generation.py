@@ -6,6 +6,8 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from .. import ops
+
 
 def sample_next(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 50, top_p: float = 0.9,
                 do_sample: bool = True) -> torch.Tensor:
@@ -41,16 +43,27 @@ class GenerationMixin:
         top_p: float = 0.9,
         do_sample: bool = True,
         eos_token_id: Optional[int] = None,
+        min_p: float = 0.0,
+        uniforms: Optional[torch.Tensor] = None,
     ) -> torch.Tensor:
         """Autoregressive sampling with a cache; stops when every sequence of the batch has just
-        produced the end token (the config's, unless given here; none if neither has one)."""
+        produced the end token (the config's, unless given here; none if neither has one).
+        `uniforms` (fp32 [max_new_tokens, B], in [0, 1)): tokens are drawn from these numbers by
+        ``ops.sample_tokens`` instead of torch's generator; min_p asks for that too and draws
+        its own numbers unless they are given."""
+        if min_p > 0.0 and uniforms is None:
+            uniforms = torch.rand(max_new_tokens, input_ids.shape[0], device=input_ids.device)
         eos = getattr(self.config, "eos_token_id", None) if eos_token_id is None else eos_token_id
         cache = None
-        for _ in range(max_new_tokens):
+        for i in range(max_new_tokens):
             step_ids = input_ids if cache is None else input_ids[:, -1:]
             out = self.forward(step_ids, past_key_values=cache, use_cache=True)
             cache = out.past_key_values
-            nxt = sample_next(out.logits[:, -1, :], temperature, top_k, top_p, do_sample)
+            if uniforms is None:
+                nxt = sample_next(out.logits[:, -1, :], temperature, top_k, top_p, do_sample)
+            else:
+                nxt = ops.sample_tokens(out.logits[:, -1, :], uniforms[i], temperature if do_sample else 0.0, top_k, top_p,
+                                        min_p)[0][:, None]
             input_ids = torch.cat([input_ids, nxt], dim=-1)
             if eos is not None and bool((nxt == eos).all()):
                 break

@@ -23,6 +23,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..core.attention import StaticKVCache
+from ..core.paged import PagedKVCache
 from ..core.layer import MuClampRequest, SplitStream, TransformerBlock
 from ..core.normalization import RMSNorm
 from .config import ComplexityConfig
@@ -176,6 +177,14 @@ class ComplexityModel(nn.Module, GenerationMixin):
         c, w = self.config, self.embed_tokens.weight
         return StaticKVCache(c.num_hidden_layers, batch, c.num_key_value_heads,
                              c.hidden_size // c.num_attention_heads, capacity, w.device, dtype=w.dtype)
+
+    def make_paged_cache(self, slots: int, pages: int, page: int = 64, max_rows: int = 2048,
+                         max_positions: Optional[int] = None, statistics: bool = False) -> PagedKVCache:
+        """Cache in pages for sequences of different lengths (see ``PagedDecoder``); max_positions: the longest that a
+        sequence gets, its evicted rows included (max_rows unless given)."""
+        c = self.config
+        return PagedKVCache(c.num_hidden_layers, slots, c.num_key_value_heads, c.hidden_size // c.num_attention_heads, pages, page,
+                            max_rows, max_positions or max_rows, self.embed_tokens.weight.device, statistics)
 
     # ------------------------------------------------------------------ utilities
     def num_parameters(self, trainable_only: bool = True) -> int:

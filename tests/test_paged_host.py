@@ -101,3 +101,80 @@ def test_wrappers_have_no_cpu_path():
         ops.evict_rows_(pool, pool, table, n, n, stat, pos, 8, 2)
     with pytest.raises(RuntimeError):
         ops.sample_tokens(torch.zeros(1, 10), torch.zeros(1))
+
+
+# --------------------------------------------------------------------------- bookkeeping of the cache
+def _prompt(rows, layers=2, hkv=2, dim=8):
+    g = torch.Generator().manual_seed(rows)
+    return [tuple(torch.randn(1, hkv, rows, dim, generator=g).to(torch.bfloat16) for _ in range(2)) for _ in range(layers)]
+
+
+def _held(cache, slot, n):
+    ids = cache.table[slot, : -(-n // cache.page)].long()
+    return cache.k[:, ids].transpose(1, 2).flatten(2, 3)[:, :, :n]
+
+
+def test_cache_takes_over_grows_and_frees():
+    from complexity_deep_b200.core.paged import PagedKVCache
+    cache = PagedKVCache(2, 3, 2, 8, pages=6, page=16, max_rows=48, max_positions=60, device="cpu", statistics=True)
+    a, b = _prompt(16), _prompt(20)
+    cache.weights.fill_(9.0)
+    s0, s1 = cache.add(a), cache.add(b)
+    assert (s0, s1, cache.free_pages) == (0, 1, 3) and cache.lengths.tolist() == [16, 20, -1] == [cache.length(i) for i in range(3)]
+    assert torch.equal(_held(cache, 0, 16), torch.stack([p[0][0] for p in a])) and torch.equal(_held(cache, 1, 20), torch.stack([p[0][0] for p in b]))
+    assert bool((cache.weights[:, 1, :, :20] == 0).all()) and bool((cache.weights[:, 1, :, 20:] == 9).all())
+    assert cache.row_positions[0, 1, 0, :20].tolist() == list(range(20))
+    cache.reserve()                                           # slot 0 has filled its page, slot 1 has room
+    assert cache.free_pages == 2 and int(cache.table[0, 1]) < 6 and int(cache.table[0, 2]) == 6
+    for _ in range(12):
+        cache.reserve()
+        cache.advance()
+    assert cache.lengths.tolist() == [28, 32, -1] and cache.positions.tolist() == [28, 32, 0]
+    cache.reserve()
+    assert cache.free_pages == 1 and len(set(cache.table[cache.table < 6].tolist())) == 5
+    cache.release(0)
+    assert cache.free_pages == 3 and cache.lengths.tolist() == [-1, 32, -1] and cache.table[0].tolist() == [6, 6, 6]
+    cache.advance()
+    assert cache.lengths.tolist() == [-1, 33, -1]             # slots that are not in use stay as they are
+    assert cache.add(_prompt(40)) == 0 and cache.free_pages == 0
+    with pytest.raises(RuntimeError):
+        cache.add(_prompt(3))
+    with pytest.raises(ValueError):
+        cache.release(2)
+
+
+def test_cache_limits():
+    from complexity_deep_b200.core.paged import PagedKVCache
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 1, 1, 8, pages=1, page=24, max_rows=8, max_positions=8, device="cpu")
+    cache = PagedKVCache(2, 1, 2, 8, pages=3, page=16, max_rows=20, max_positions=40, device="cpu")
+    with pytest.raises(ValueError):
+        cache.add(_prompt(21))
+    cache.add(_prompt(19))
+    cache.reserve()
+    cache.advance()
+    assert cache.full()
+    with pytest.raises(RuntimeError, match="rows"):
+        cache.reserve()
+    with pytest.raises(RuntimeError, match="statistics"):
+        cache.evict(8, 2)
+
+
+def test_cache_bookkeeping_of_an_eviction(monkeypatch):
+    from complexity_deep_b200.core import paged
+    cache = paged.PagedKVCache(2, 2, 2, 8, pages=8, page=16, max_rows=64, max_positions=64, device="cpu", statistics=True)
+    cache.add(_prompt(60))
+    cache.add(_prompt(18))
+    calls = []
+    monkeypatch.setattr(paged.ops, "evict_rows_", lambda *a: calls.append(a[-2:]))
+    cache.evict(20, 4)
+    assert calls == [(20, 4)] and cache.lengths.tolist() == [20, 18] == [cache.length(0), cache.length(1)] and cache.free_pages == 4
+    assert int(cache.table[0, 1]) < 8 and cache.table[0, 2:].tolist() == [8, 8] and cache.positions.tolist() == [60, 18]
+
+
+def test_command_line_prompts():
+    from complexity_deep_b200 import cli
+    assert cli.parse_prompts(["1,2", "3"], equal=False) == [[1, 2], [3]]
+    for texts, equal in ((["1,2", "3"], True), (["1", ""], False)):
+        with pytest.raises(SystemExit):
+            cli.parse_prompts(texts, equal)
