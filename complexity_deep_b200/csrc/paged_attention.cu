@@ -849,11 +849,13 @@ int cluster_of(long long pairs, long long tiles) {
 
 // Where things lie in the workspace.
 struct Layout {
+  int cluster;
   long long tiles;        // of a pair
   size_t part, tile_rows, top_sum, scores, bytes;
 };
 Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
   Layout l = {};
+  l.cluster = cluster_of(static_cast<long long>(B) * hkv, (static_cast<long long>(width) * page + kTile - 1) / kTile);
   auto take = [&](size_t n) {
     const size_t at = l.bytes;
     l.bytes += (n + 255) / 256 * 256;
@@ -861,10 +863,12 @@ Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
   };
   const long long rows = static_cast<long long>(width) * page, pairs = static_cast<long long>(B) * hkv;
   l.tiles = (rows + kTile - 1) / kTile;
-  take(sizeof(Stretch) * kMostBlocks);
-  l.part = take(sizeof(float) * kMostBlocks * 2 * G * (D + 2));
-  l.tile_rows = weights ? take(sizeof(int4) * l.tiles * pairs) : 0;
-  l.top_sum = weights ? take(sizeof(float2) * pairs * G) : 0;
+  if (!l.cluster) {
+    take(sizeof(Stretch) * kMostBlocks);
+    l.part = take(sizeof(float) * kMostBlocks * 2 * G * (D + 2));
+    l.tile_rows = weights ? take(sizeof(int4) * l.tiles * pairs) : 0;
+    l.top_sum = weights ? take(sizeof(float2) * pairs * G) : 0;
+  }
   l.scores = weights ? take(sizeof(float) * l.tiles * pairs * G * kTile) : 0;
   return l;
 }
@@ -925,7 +929,7 @@ cudaError_t launch_paged_attention(const cd_paged& c, const cd_paged_step* step,
   a.out = static_cast<bf16*>(out);
   a.status = status;
   a.pair_tiles = l.tiles;
-  a.cluster = cluster_of(static_cast<long long>(B) * hkv, l.tiles);
+  a.cluster = l.cluster;
   a.stretches = reinterpret_cast<Stretch*>(base);
   a.part = reinterpret_cast<float*>(base + l.part);
   a.tile_rows = reinterpret_cast<int4*>(base + l.tile_rows);

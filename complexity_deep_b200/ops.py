@@ -1396,9 +1396,8 @@ def combine_top_(stream: torch.Tensor, y: torch.Tensor, inv_perm: torch.Tensor, 
 
 # --------------------------------------------------------------------------- paged cache
 def _on(t: torch.Tensor, name: str, dtype, device: int, shape) -> int:
-    """Address of a contiguous CUDA tensor of that type, device index and shape."""
-    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda
-            and t.get_device() == device):
+    """Address of a contiguous CUDA tensor of that type, device index (a CPU tensor's is -1) and shape."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
         return t.data_ptr()
     raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {list(shape)} on cuda:{device}")
 
@@ -1414,62 +1413,62 @@ def _here(t: torch.Tensor, name: str) -> int:
 
 
 def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
-           weights: Optional[torch.Tensor], layers: int, batch: int, device: int) -> _lib.Paged:
+           weights: Optional[torch.Tensor], batch: int, device: int) -> _lib.Paged:
     """The cache as the library takes it; pools [pages, kv heads, page, D], of several layers with the layers in front."""
     shape, strides = k_pages.shape, k_pages.stride()
-    pages, hkv, page, _ = shape[-4:]
+    *layers, pages, hkv, page, _ = shape
     stride_p, stride_h, stride_t, stride_d = strides[-4:]
-    k, v = k_pages.data_ptr(), v_pages.data_ptr()
     if (k_pages.dtype is not BF16 or v_pages.dtype is not BF16 or stride_d != 1 or v_pages.shape != shape
-            or v_pages.stride() != strides or not (k_pages.is_cuda and v_pages.is_cuda)
-            or not k_pages.get_device() == device == v_pages.get_device()):
+            or v_pages.stride() != strides or not k_pages.get_device() == device == v_pages.get_device()):
         raise RuntimeError(f"pages: expected bf16 [pages, kv heads, page, D] on cuda:{device}, D contiguous, keys and values with the "
                            "same shape and strides")
+    k, v = k_pages.data_ptr(), v_pages.data_ptr()
     if (stride_p | stride_h | stride_t | strides[0]) & 7 or (k | v) & 15:
         raise RuntimeError("pages: strides must be multiples of 8 elements, the pools lie on 16-byte boundaries")
-    if (block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] < 1
-            or block_table.stride(1) != 1 or not block_table.is_cuda or block_table.get_device() != device):
+    table = block_table.shape
+    if (block_table.dtype is not torch.int32 or len(table) != 2 or table[0] != batch or table[1] < 1 or block_table.stride(1) != 1
+            or block_table.get_device() != device):
         raise RuntimeError(f"block_table: expected int32 [{batch}, pages of a sequence] on cuda:{device}")
-    width = block_table.shape[1]
-    w = None
-    if weights is not None:
-        w = _on(weights, "weights", torch.float32, device,
-                (layers, batch, hkv, width * page) if len(shape) == 5 else (batch, hkv, width * page))
+    width = table[1]
     return _lib.Paged(k, v, stride_p, stride_h, stride_t, block_table.data_ptr(), block_table.stride(0),
-                      _on(lengths, "lengths", torch.int32, device, (batch,)), w, pages, page, width)
+                      _on(lengths, "lengths", torch.int32, device, (batch,)),
+                      None if weights is None else _on(weights, "weights", torch.float32, device, (*layers, batch, hkv, width * page)),
+                      pages, page, width)
 
 
+# sizes of workspaces: asked for once per shape and device
 @functools.lru_cache(maxsize=256)
-def _paged_workspace(*sizes) -> int:
+def _paged_workspace(device: int, *sizes) -> int:
     return _lib.load().cd_paged_attention_workspace_bytes(*sizes)
 
 
 @functools.lru_cache(maxsize=256)
-def _evict_workspace(*sizes) -> int:
+def _evict_workspace(device: int, *sizes) -> int:
     return _lib.load().cd_evict_rows_workspace_bytes(*sizes)
 
 
-def _attend_paged(step, c: _lib.Paged, q: torch.Tensor, hq: int, hkv: int, D: int) -> torch.Tensor:
+def _attend_paged(step, c: _lib.Paged, q: torch.Tensor, batch: int, hq: int, hkv: int, D: int, device: int) -> torch.Tensor:
     lib = _lib.load()
-    B = q.shape[0]
-    out = q.new_empty(B, hq * D)
-    n = _paged_workspace(B, hq, hkv, D, c.page, c.width, 0 if c.weights is None else 1)
-    ws = q.new_empty(n // 2)
+    out = q.new_empty(batch, hq * D)
+    n = _paged_workspace(device, batch, hq, hkv, D, c.page, c.width, 0 if c.weights is None else 1)
+    ws = q.new_empty(n // 2) if n else None
     with _Span("paged_attention", 2):
         if step is None:
-            status = lib.cd_paged_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), D ** -0.5, B, hq, hkv, D, out.data_ptr(),
-                                            ws.data_ptr(), n, _stream())
+            status = lib.cd_paged_attention(ctypes.byref(c), q.data_ptr(), q.stride(0), D ** -0.5, batch, hq, hkv, D, out.data_ptr(),
+                                            _ptr(ws), n, _stream())
         else:
-            status = lib.cd_paged_step_attention(ctypes.byref(c), ctypes.byref(step), q.data_ptr(), D ** -0.5, B, hq, hkv, D,
-                                                 out.data_ptr(), ws.data_ptr(), n, _stream())
-    _lib.check(status, "cd_paged_attention" if step is None else "cd_paged_step_attention")
+            status = lib.cd_paged_step_attention(ctypes.byref(c), ctypes.byref(step), q.data_ptr(), D ** -0.5, batch, hq, hkv, D,
+                                                 out.data_ptr(), _ptr(ws), n, _stream())
+    if status:
+        _lib.check(status, "cd_paged_attention" if step is None else "cd_paged_step_attention")
     return out
 
 
 def _heads(k_pages: torch.Tensor, hq: int, hkv: int, head_dim: int) -> None:
-    if head_dim not in (64, 128) or hkv < 1 or hq < 1 or hq % hkv or hq // hkv > 16:
+    if (head_dim != 64 and head_dim != 128) or hkv < 1 or hq < 1 or hq % hkv or hq // hkv > 16:
         raise RuntimeError("paged attention needs head size 64 or 128 and at most 16 query heads per KV head")
-    if k_pages.dim() != 4 or k_pages.shape[1] != hkv or k_pages.shape[3] != head_dim or k_pages.shape[2] not in (16, 32, 64, 128, 256):
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[1] != hkv or shape[3] != head_dim or shape[2] not in (16, 32, 64, 128, 256):
         raise RuntimeError(f"pages: expected [pages, {hkv}, 16 / 32 / 64 / 128 / 256 rows, {head_dim}]")
 
 
@@ -1486,8 +1485,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.dtype is not BF16 or q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < hq * head_dim or q.stride(0) % 8 or q.data_ptr() & 15:
         raise RuntimeError("q: expected bf16 rows of at least hq * head_dim elements on 16-byte boundaries")
     forward_only(q, "paged_attention")
-    c = _paged(k_pages, v_pages, block_table, lengths, weights, 1, q.shape[0], device)
-    return _attend_paged(None, c, q, hq, hkv, head_dim)
+    B = q.shape[0]
+    c = _paged(k_pages, v_pages, block_table, lengths, weights, B, device)
+    return _attend_paged(None, c, q, B, hq, hkv, head_dim, device)
 
 
 def paged_step_attention(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor], cos: torch.Tensor,
@@ -1506,11 +1506,9 @@ def paged_step_attention(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Op
     forward_only(qkv, "paged_step_attention")
     if (q_w is None) != (k_w is None):
         raise RuntimeError("norm weights: both or none")
-    c = _paged(k_pages, v_pages, block_table, lengths, weights, 1, B, device)
-    rows = c.width * c.page
-    if cos.dim() != 2:
-        raise RuntimeError("cos/sin: expected [positions, head_dim]")
-    table = (cos.shape[0], D)
+    c = _paged(k_pages, v_pages, block_table, lengths, weights, B, device)
+    positions_held = cos.shape[0] if cos.dim() else 0
+    table = (positions_held, D)
     if (cos.data_ptr() | sin.data_ptr()) & 7:
         cos, sin = cos.clone(), sin.clone()
     if q_w is not None and q_w.data_ptr() & 3:
@@ -1520,10 +1518,10 @@ def paged_step_attention(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Op
         None if k_w is None else _on(k_w, "k_norm.weight", BF16, device, (D,)),
         _on(cos, "cos", torch.float32, device, table), _on(sin, "sin", torch.float32, device, table),
         _on(positions, "positions", torch.int32, device, (B,)),
-        None if row_positions is None else _on(row_positions, "row_positions", torch.int32, device, (B, hkv, rows)),
-        float(eps), cos.shape[0])
+        None if row_positions is None else _on(row_positions, "row_positions", torch.int32, device, (B, hkv, c.width * c.page)),
+        float(eps), positions_held)
     _on(qkv, "qkv", BF16, device, (B, (hq + 2 * hkv) * D))
-    return _attend_paged(step, c, qkv, hq, hkv, D)
+    return _attend_paged(step, c, qkv, B, hq, hkv, D, device)
 
 
 def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -1549,7 +1547,7 @@ def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     if (weights_out is None) != (row_positions_out is None):
         raise RuntimeError("evict_rows_: both outputs or none")
     B = block_table.shape[0]
-    c = _paged(k_pages, v_pages, block_table, lengths, weights, layers, B, device)
+    c = _paged(k_pages, v_pages, block_table, lengths, weights, B, device)
     shape = weights.shape
     if weights_out is None:
         weights_out, row_positions_out = weights, row_positions
@@ -1558,7 +1556,7 @@ def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
                    _on(weights_out, "weights_out", torch.float32, device, shape),
                    _on(row_positions_out, "row_positions_out", torch.int32, device, shape), keep, recent)
     lib = _lib.load()
-    n = _evict_workspace(layers, B, hkv, c.page, c.width, keep)
+    n = _evict_workspace(device, layers, B, hkv, c.page, c.width, keep)
     ws = k_pages.new_empty(n // 2) if n else None
     with _Span("evict_rows"):
         _lib.check(lib.cd_evict_rows(ctypes.byref(c), ctypes.byref(e), layers, k_pages.stride(0) if k_pages.dim() == 5 else 0, B, hkv, D,
@@ -1581,16 +1579,19 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     B, V = logits.shape
     if V > 1 << 18:
         raise RuntimeError("sample_tokens: at most 262144 logits a row")
-    r = _lib.Sample(uniform=_on(uniform, "uniform", torch.float32, device, (B,)))
-    for name, rule, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                              ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    each = [None, None, None, None]                       # tensors' addresses; the numbers of the others
+    one = [1.0, 1.0, 0.0, 0]
+    for i, rule in enumerate((temperature, top_p, min_p, top_k)):
         if isinstance(rule, torch.Tensor):
-            setattr(r, name + "s", _on(rule, name, dtype, device, (B,)))
+            each[i] = _on(rule, ("temperature", "top_p", "min_p", "top_k")[i], torch.float32 if i < 3 else torch.int32, device, (B,))
         else:
-            setattr(r, name, rule)
+            one[i] = rule
+    r = _lib.Sample(_on(uniform, "uniform", torch.float32, device, (B,)), *each, *one)
     ids, probs = uniform.new_empty(B, dtype=torch.int64), uniform.new_empty(B)
     if B:
         with _Span("sample_tokens"):
-            _lib.check(_lib.load().cd_sample_tokens(logits.data_ptr(), int(logits.dtype is torch.float32), logits.stride(0), B, V,
-                                                    ctypes.byref(r), ids.data_ptr(), probs.data_ptr(), _stream()), "cd_sample_tokens")
+            status = _lib.load().cd_sample_tokens(logits.data_ptr(), 0 if logits.dtype is BF16 else 1, logits.stride(0), B, V,
+                                                  ctypes.byref(r), ids.data_ptr(), probs.data_ptr(), _stream())
+        if status:
+            _lib.check(status, "cd_sample_tokens")
     return ids, probs
