@@ -19,9 +19,10 @@
 // The share of a row in its softmax is known only when the pair's maximum and sum are: where weights are asked for, scores are
 // left in the workspace and the second kernel turns them into shares (clusters do so themselves, when their sums have met).
 //
-// A step (kStep) brings the raw projections: a warp normalises and rotates the query heads where it needs them, in the registers that
-// the products take; the block that has the pair's last tile does so for the key, writes key and value into the new row's place, in
-// the cache and in its copy of the tile.
+// A sixth warp prepares the next pair while the tiles of this one are taken: the query heads as operand fragments, of a step
+// (kStep) normalised and rotated from the raw projections, and, where the block has the pair's last tile, the new key and value, which
+// it writes into the cache and the warp that has the row puts into its copy of the tile. Doing this in the four warps, between
+// pairs, cost 2 to 3 us a pair.
 #include <cfloat>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -36,8 +37,9 @@ namespace cdeep {
 namespace {
 
 constexpr int kTile = 64;                 // rows of a tile
-constexpr int kWarps = 4;                 // that compute; one more feeds them
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kWarps = 4;                 // that compute; one more feeds them, one prepares pairs
+constexpr int kThreads = 32 * (kWarps + 2);
+constexpr int kSlots = kWarps / 2;        // in which warps hand over their sums
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMostCluster = 8;           // blocks of a pair
 constexpr int kClusterTiles = 8;          // tiles of a block, up to which pairs have clusters
@@ -45,22 +47,25 @@ constexpr int kClusterTiles = 8;          // tiles of a block, up to which pairs
 __host__ __device__ constexpr int stage_bytes(int D) { return 2 * kTile * D * 2; }
 // floats of a lane that a warp hands over: its columns of each head it holds
 __host__ __device__ constexpr int lane_floats(int D, bool wide) { return D / 8 * (wide ? 4 : 2); }
-__host__ __device__ constexpr int merge_bytes(int D, bool wide) { return (kWarps - 1) * 32 * (lane_floats(D, wide) + 4) * 4; }
+__host__ __device__ constexpr int merge_bytes(int D, bool wide) { return kSlots * 32 * (lane_floats(D, wide) + 4) * 4; }
+// operand fragments of a pair's query heads, then the new row's key and value
+__host__ __device__ constexpr int query_bytes(int D, bool wide) { return D / 16 * 32 * 16 * (wide ? 2 : 1) + 2 * D * 2; }
 // Two blocks an SM (113 KB each): one computes while the other starts a pair or ends one. 16 heads of 128 leave room for one.
 __host__ __device__ constexpr int blocks_per_sm(int D, bool wide) { return wide && D == 128 ? 1 : 2; }
 __host__ __device__ constexpr int stages_of(int D, bool wide) {
-  return (232448 / blocks_per_sm(D, wide) - 1024 * 3 - merge_bytes(D, wide)) / stage_bytes(D);
+  return (232448 / blocks_per_sm(D, wide) - 1024 * 2 - 512 - merge_bytes(D, wide) - query_bytes(D, wide)) / stage_bytes(D);
 }
 __host__ __device__ constexpr int smem_bytes(int D, bool wide) {
-  return 1024 + stages_of(D, wide) * stage_bytes(D) + merge_bytes(D, wide);
+  return 1024 + stages_of(D, wide) * stage_bytes(D) + merge_bytes(D, wide) + query_bytes(D, wide);
 }
 
-// For the second kernel: a block's stretch and the pairs at its ends.
+// For the second kernel: a block's stretch and the pairs at its ends, all that it has to know before it can ask for anything.
 struct End {
-  int pair, unit;         // its first tile in the line
+  int pair;
   int first, last;        // blocks that have tiles of it
+  int second;             // whether the first of them had begun with another pair
 };
-struct Stretch {
+struct __align__(16) Stretch {
   int blocks, begins, ends, pad;          // blocks that have one; this block's tiles
   End end[2];
 };
@@ -79,11 +84,14 @@ struct Args {
   long long pair_tiles;   // that a pair has room for
   // workspace
   Stretch* stretches;     // [blocks of the grid]
-  float* part;            // [blocks][2][G (D + 2)]: of the first pair of a block and of the last
+  float* part;            // [blocks][2][G D + 2 G, to a multiple of four]: of the first pair of a block and of the last
   int4* tile_rows;        // [tiles] pair, first row, rows of the sequence; this and the next two where weights are asked for
   float2* top_sum;        // [B hkv][G] maximum and 1 / sum of pairs that are not cut
   float* scores;          // [tiles][G][64], times log2 e
 };
+
+// Floats of a part: the heads' columns, then their maxima and sums.
+__host__ __device__ constexpr int part_floats(int G, int D) { return (G * (D + 2) + 3) / 4 * 4; }
 
 // Equal stretches of a line of `units` tiles: the first ones are a tile longer where it does not divide.
 struct Line {
@@ -196,30 +204,43 @@ __device__ __forceinline__ void load_head(const Args& a, const bf16* x, bool the
   }
 }
 
-// The new row's key, normalised and rotated: lane l holds columns 32 i + l.
+// The new row's key, normalised and rotated, and value: lane l holds columns 32 i + l. What it takes is asked for first.
 template <int D>
-__device__ __forceinline__ void new_key(const Args& a, const bf16* x, int pos, int lane, bf16 (&y)[D / 32]) {
-  constexpr int N = D / 32;
-  float v[N], ss = 0.f;
+struct NewRow {
+  static constexpr int N = D / 32;
+  bf16 x[N], w[N], value[N];
+  float cs[N], sn[N];
+  __device__ __forceinline__ void load(const Args& a, const bf16* key, const bf16* val, int pos, int lane) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = to_f32(x[lane + 32 * i]);
-    ss += v[i] * v[i];
+    for (int i = 0; i < N; ++i) {
+      x[i] = key[lane + 32 * i];
+      value[i] = val[lane + 32 * i];
+      w[i] = a.st.k_w ? static_cast<const bf16*>(a.st.k_w)[lane + 32 * i] : bf16();
+      cs[i] = a.st.cos_t[static_cast<long long>(pos) * D + lane + 32 * i];
+      sn[i] = a.st.sin_t[static_cast<long long>(pos) * D + lane + 32 * i];
+    }
   }
+  __device__ __forceinline__ void key(const Args& a, bf16 (&y)[N]) const {
+    float v[N], ss = 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (a.st.k_w) {
-    const float r = rsqrtf(ss / D + a.st.eps);
+    for (int i = 0; i < N; ++i) {
+      v[i] = to_f32(x[i]);
+      ss += v[i] * v[i];
+    }
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= r * to_f32(static_cast<const bf16*>(a.st.k_w)[lane + 32 * i]);
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (a.st.k_w) {
+      const float r = rsqrtf(ss / D + a.st.eps);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] *= r * to_f32(w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float other = i < N / 2 ? -v[i + N / 2] : v[i - N / 2];
+      y[i] = from_f32<bf16>(v[i] * cs[i] + other * sn[i]);
+    }
   }
-  const float *cs = a.st.cos_t + static_cast<long long>(pos) * D + lane, *sn = a.st.sin_t + static_cast<long long>(pos) * D + lane;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float other = i < N / 2 ? -v[i + N / 2] : v[i - N / 2];
-    y[i] = from_f32<bf16>(v[i] * cs[32 * i] + other * sn[32 * i]);
-  }
-}
+};
 
 // Byte of column x of row r within a tile: halves of 64 columns, rows of 128 bytes, 16-byte pieces exchanged by the row (as TMA does).
 __device__ __forceinline__ uint32_t place(int r, int x) { return (x >> 6) * (kTile * 128) + r * 128 + ((((x >> 3) & 7) ^ (r & 7)) << 4) + (x & 7) * 2; }
@@ -285,7 +306,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int kHeads = kWide ? 2 : 1;                   // of a lane
   constexpr int kFloats = lane_floats(D, kWide);
   extern __shared__ unsigned char s_dyn[];
-  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_query, s_query_taken;
   __shared__ int s_scan[kThreads / 32];
   __shared__ Walk s_start;
   __shared__ float2 s_final[16];                          // maximum and 1 / sum of a pair's heads
@@ -293,6 +314,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __shared__ int s_abort;
   unsigned char* ring = s_dyn + ((1024 - (smem_u32(s_dyn) & 1023)) & 1023);
   float* s_merge = reinterpret_cast<float*>(ring + kStages * stage_bytes(D));
+  uint4* s_heads = reinterpret_cast<uint4*>(ring + kStages * stage_bytes(D) + merge_bytes(D, kWide));
+  bf16* s_new = reinterpret_cast<bf16*>(s_heads + D / 16 * 32 * (kWide ? 2 : 1));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int block = blockIdx.x;
 
@@ -301,6 +324,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       mbar_init(&s_full[s], 1);
       mbar_init(&s_empty[s], kWarps);
     }
+    mbar_init(&s_query, 1);
+    mbar_init(&s_query_taken, kWarps);
     fence_barrier_init();
     s_abort = 0;
     tma_prefetch_desc(&k_map);
@@ -423,22 +448,18 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     }
     if (!kCluster) return;
   }
-
-  // ---------------------------------------------------------------------- computes
-  const int g0 = lane >> 2, col = 2 * (lane & 3);
-  const long long unit0 = unit;
-  bool handed = false;                                    // the buffers of the warps' sums are in use
-  bool first_pair = true;
-  while (warp < kWarps && (kCluster || w.left > 0)) {
-    const int tiles = tiles_of(w.rows), take = min(tiles - w.t, w.left);
-    const int pair = w.b * a.hkv + w.h;
-    const bool last_tile = w.t + take == tiles && take > 0;
-    int pos = 0;
-    if constexpr (kStep) pos = a.st.positions[w.b];
-    const bf16* q = a.q + w.b * a.q_stride;
-    // the query heads: what bf16 holds of them and what it cuts off
-    uint32_t qh[D / 16][4], ql[kWide ? D / 16 : 1][4];
-    {
+  if (warp == kWarps + 1) {
+    // ------------------------------------------------------------------ prepares pairs
+    for (int turn = 0; w.left > 0; turn ^= 1) {
+      const int tiles = tiles_of(w.rows), take = min(tiles - w.t, w.left), g0 = lane >> 2;
+      const bool last_tile = w.t + take == tiles;
+      const bf16* q = a.q + w.b * a.q_stride;
+      const int pos = kStep ? a.st.positions[w.b] : 0;
+      NewRow<D> row;
+      if (kStep && last_tile)
+        row.load(a, q + static_cast<long long>(a.hkv * a.G + w.h) * D, q + static_cast<long long>(a.hkv * (a.G + 1) + w.h) * D, pos, lane);
+      // what bf16 holds of the heads and what it cuts off
+      uint4 part[D / 16][kWide ? 2 : 1];
       float v[D / 16][4];
       load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0) * D, g0 < a.G, pos, lane, v);
 #pragma unroll
@@ -446,49 +467,92 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         uint32_t hi[2], lo[2];
         split_pair(v[k][0], v[k][1], hi[0], lo[0]);
         split_pair(v[k][2], v[k][3], hi[1], lo[1]);
-        qh[k][0] = hi[0];
-        qh[k][2] = hi[1];
-        if constexpr (kWide) {
-          ql[k][0] = lo[0];
-          ql[k][2] = lo[1];
-        } else {
-          qh[k][1] = lo[0];
-          qh[k][3] = lo[1];
-        }
+        part[k][0] = kWide ? make_uint4(hi[0], 0, hi[1], 0) : make_uint4(hi[0], lo[0], hi[1], lo[1]);
+        if constexpr (kWide) part[k][1] = make_uint4(lo[0], 0, lo[1], 0);
       }
       if constexpr (kWide) {
         load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0 + 8) * D, g0 + 8 < a.G, pos, lane, v);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          split_pair(v[k][0], v[k][1], qh[k][1], ql[k][1]);
-          split_pair(v[k][2], v[k][3], qh[k][3], ql[k][3]);
+          split_pair(v[k][0], v[k][1], part[k][0].y, part[k][1].y);
+          split_pair(v[k][2], v[k][3], part[k][0].w, part[k][1].w);
         }
       }
-    }
-    // the new row, by the warp whose rows include it
-    const int new_row = w.rows - 1;
-    const bool owner = kStep && last_tile && (new_row % kTile) / 16 == warp;
-    bf16 nk[D / 32], nv[D / 32];
-    if (kStep && owner) {
-      new_key<D>(a, q + static_cast<long long>(a.hkv * a.G + w.h) * D, pos, lane, nk);
-      const bf16* value = q + static_cast<long long>(a.hkv * (a.G + 1) + w.h) * D;
-      const long long at = a.c.table[w.b * a.c.table_stride + new_row / a.c.page] * a.c.stride_p + w.h * a.c.stride_h +
-                           new_row % a.c.page * a.c.stride_t;
+      bf16 key[D / 32];
+      if (kStep && last_tile) {
+        row.key(a, key);
+        const int at = w.rows - 1;
+        const long long to = a.c.table[w.b * a.c.table_stride + at / a.c.page] * a.c.stride_p + w.h * a.c.stride_h + at % a.c.page * a.c.stride_t;
+        // the tile's copy of this row may be of before or after: it is replaced
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) nv[i] = value[lane + 32 * i];
-      if (lane == 0 && a.st.row_positions)
-        a.st.row_positions[static_cast<long long>(pair) * a.c.width * a.c.page + new_row] = pos;
-      // the tile's copy is under way or has arrived: whatever it holds of this row is replaced below
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        static_cast<bf16*>(a.c.k)[at + lane + 32 * i] = nk[i];
-        static_cast<bf16*>(a.c.v)[at + lane + 32 * i] = nv[i];
+        for (int i = 0; i < D / 32; ++i) {
+          static_cast<bf16*>(a.c.k)[to + lane + 32 * i] = key[i];
+          static_cast<bf16*>(a.c.v)[to + lane + 32 * i] = row.value[i];
+        }
+        if (lane == 0 && a.st.row_positions)
+          a.st.row_positions[(static_cast<long long>(w.b) * a.hkv + w.h) * a.c.width * a.c.page + at] = pos;
       }
+      if (!mbar_wait(&s_query_taken, turn ^ 1, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+        for (int i = 0; i < (kWide ? 2 : 1); ++i) s_heads[(k * (kWide ? 2 : 1) + i) * 32 + lane] = part[k][i];
+      }
+      if (kStep && last_tile) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          s_new[lane + 32 * i] = key[i];
+          s_new[D + lane + 32 * i] = row.value[i];
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_query);
+      next_pair<kStep>(a, w, take);
+    }
+    if (!kCluster) return;
+  }
+
+  // ---------------------------------------------------------------------- computes
+  const int g0 = lane >> 2, col = 2 * (lane & 3);
+  const long long unit0 = unit;
+  bool handed = false;                                    // the buffers of the warps' sums are in use
+  bool first_pair = true;
+  int query_phase = 0;
+  while (warp < kWarps && (kCluster || w.left > 0)) {
+    const int tiles = tiles_of(w.rows), take = min(tiles - w.t, w.left);
+    const int pair = w.b * a.hkv + w.h;
+    const bool last_tile = w.t + take == tiles && take > 0;
+    uint32_t qh[D / 16][4], ql[kWide ? D / 16 : 1][4];
+    const int new_row = w.rows - 1;
+    const bool owner = kStep && last_tile && (new_row % kTile) / 16 == warp;   // of the new row: the warp whose rows include it
+    bf16 nk[D / 32], nv[D / 32];
+    if (take > 0) {
+      if (!mbar_wait(&s_query, query_phase, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
+      query_phase ^= 1;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint4 hi = s_heads[k * (kWide ? 2 : 1) * 32 + lane];
+        qh[k][0] = hi.x, qh[k][1] = hi.y, qh[k][2] = hi.z, qh[k][3] = hi.w;
+        if constexpr (kWide) {
+          const uint4 lo = s_heads[(2 * k + 1) * 32 + lane];
+          ql[k][0] = lo.x, ql[k][1] = lo.y, ql[k][2] = lo.z, ql[k][3] = lo.w;
+        }
+      }
+      if (owner) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          nk[i] = s_new[lane + 32 * i];
+          nv[i] = s_new[D + lane + 32 * i];
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_query_taken);
     }
     if (!kCluster && tid == 0 && (first_pair || take == w.left)) {
       const Line line(units, blocks);
       const int at = static_cast<int>(unit) - w.t;
-      const End end = {pair, at, line.block_of(at), line.block_of(at + tiles - 1)};
+      const int first = line.block_of(at);
+      const End end = {pair, first, line.block_of(at + tiles - 1), line.first(first) < at ? 1 : 0};
       if (first_pair) a.stretches[block].end[0] = end;
       if (take == w.left) a.stretches[block].end[1] = end;
     }
@@ -631,43 +695,46 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
-    if (handed) warps_sync();                             // the first warp has read the last pair's
+    if (handed) warps_sync();                             // the last pair's have been read
     handed = true;
-    if (warp > 0) {
-      float* to_first = s_merge + (warp - 1) * 32 * (kFloats + 4);
+    auto hand_over = [&](int slot) {
+      float4* to = reinterpret_cast<float4*>(s_merge + slot * 32 * (kFloats + 4));
 #pragma unroll
-      for (int x = 0; x < kFloats / 4; ++x)
-        reinterpret_cast<float4*>(to_first)[x * 32 + lane] = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
-      reinterpret_cast<float4*>(to_first)[kFloats / 4 * 32 + lane] = make_float4(m[0], l[0], m[kHeads - 1], l[kHeads - 1]);
-    }
+      for (int x = 0; x < kFloats / 4; ++x) to[x * 32 + lane] = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
+      to[kFloats / 4 * 32 + lane] = make_float4(m[0], l[0], m[kHeads - 1], l[kHeads - 1]);
+    };
+    auto take_over = [&](int slot) {
+      const float4* s = reinterpret_cast<const float4*>(s_merge + slot * 32 * (kFloats + 4));
+      const float4 ml = s[kFloats / 4 * 32 + lane];
+      float own[kHeads], its[kHeads];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const float om = i ? ml.z : ml.x, ol = i ? ml.w : ml.y, top = fmaxf(m[i], om);
+        own[i] = exp2f(m[i] - top);
+        its[i] = exp2f(om - top);
+        l[i] = l[i] * own[i] + ol * its[i];
+        m[i] = top;
+      }
+#pragma unroll
+      for (int x = 0; x < kFloats / 4; ++x) {
+        const float4 v = s[x * 32 + lane];
+        // pairs of columns: of one head, or of the lane's two in turn
+        f[4 * x] = f[4 * x] * own[0] + v.x * its[0];
+        f[4 * x + 1] = f[4 * x + 1] * own[0] + v.y * its[0];
+        f[4 * x + 2] = f[4 * x + 2] * own[kHeads - 1] + v.z * its[kHeads - 1];
+        f[4 * x + 3] = f[4 * x + 3] * own[kHeads - 1] + v.w * its[kHeads - 1];
+      }
+    };
+    if (warp >= kSlots) hand_over(warp - kSlots);
+    warps_sync();
+    if (warp < kSlots) take_over(warp);
+    if (warp == 1) hand_over(1);
     warps_sync();
     if (warp == 0) {
-#pragma unroll
-      for (int other = 0; other < kWarps - 1; ++other) {
-        const float4* s = reinterpret_cast<const float4*>(s_merge + other * 32 * (kFloats + 4));
-        const float4 ml = s[kFloats / 4 * 32 + lane];
-        float own[kHeads], its[kHeads];
-#pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-          const float om = i ? ml.z : ml.x, ol = i ? ml.w : ml.y, top = fmaxf(m[i], om);
-          own[i] = exp2f(m[i] - top);
-          its[i] = exp2f(om - top);
-          l[i] = l[i] * own[i] + ol * its[i];
-          m[i] = top;
-        }
-#pragma unroll
-        for (int x = 0; x < kFloats / 4; ++x) {
-          const float4 v = s[x * 32 + lane];
-          // pairs of columns: of one head, or of the lane's two in turn
-          f[4 * x] = f[4 * x] * own[0] + v.x * its[0];
-          f[4 * x + 1] = f[4 * x + 1] * own[0] + v.y * its[0];
-          f[4 * x + 2] = f[4 * x + 2] * own[kHeads - 1] + v.z * its[kHeads - 1];
-          f[4 * x + 3] = f[4 * x + 3] * own[kHeads - 1] + v.w * its[kHeads - 1];
-        }
-      }
+      take_over(1);
       const bool whole = w.t == 0 && last_tile;
       if constexpr (kCluster) {
-        // for the other blocks: where the second warp's sums have been, and the heads' maxima and sums
+        // for the other blocks: the columns where the third warp's have been, and the heads' maxima and sums
         float4* to_others = reinterpret_cast<float4*>(s_merge);
 #pragma unroll
         for (int x = 0; x < kFloats / 4; ++x) to_others[x * 32 + lane] = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
@@ -688,7 +755,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                   bf_pack(f[2 * kHeads * j + 2 * i] * inv, f[2 * kHeads * j + 2 * i + 1] * inv);
             if (a.scores && (lane & 3) == 0) a.top_sum[pair * a.G + g] = make_float2(m[i], inv);
           } else {
-            float* part = a.part + (2LL * block + (first_pair ? 0 : 1)) * a.G * (D + 2);
+            float* part = a.part + (2LL * block + (first_pair ? 0 : 1)) * part_floats(a.G, D);
 #pragma unroll
             for (int j = 0; j < D / 8; ++j)
               *reinterpret_cast<float2*>(part + g * D + 8 * j + col) =
@@ -759,10 +826,11 @@ constexpr int kMostBlocks = 2 * 160;
 constexpr int kFinishThreads = 256;
 
 // What a stretch has left: the pairs at its two ends where they are cut (their output, by the block behind the first cut), half of
-// the warps each; then the weights of its tiles, a warp a tile.
+// the warps each; then the weights of its tiles, a warp a tile. A chain of three loads, each for all that the one before has made
+// known: 3 us, where asking for things as they came took 9 (32 sequences, 3 600 tiles).
 template <bool kStep>
 __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args a, int D) {
-  constexpr int kHalf = kFinishThreads / 2;
+  constexpr int kHalf = kFinishThreads / 2, kAhead = 4;
   __shared__ float s_scale[2][kMostBlocks * 16];          // of a part's head
   __shared__ float2 s_final[2][16];
   griddep_wait();
@@ -770,47 +838,74 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args
   const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.G;
   const Stretch st = a.stretches[c];
   if (c >= st.blocks) return;
-  // the warp's first tile is asked for ahead of everything
+  // the first tile: scores of its first heads
   int u = st.begins + warp;
   const bool tile = a.scores && u < st.ends;
-  int4 at = tile ? a.tile_rows[u] : make_int4(-1, 0, 0, 0);
-
+  const float* scores = a.scores + static_cast<long long>(u) * G * kTile + 2 * lane;
+  int4 at = make_int4(-1, 0, 0, 0);
+  float2 ahead[kAhead];
+  if (tile) {
+    at = a.tile_rows[u];
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) ahead[g] = *reinterpret_cast<const float2*>(scores + min(g, G - 1) * kTile);
+  }
   const int half = tid >= kHalf, in_half = tid - half * kHalf;
   const End p = half ? st.end[1] : st.end[0];
   const bool cut = p.first < p.last && !(half && st.end[0].pair == p.pair);
-  const int parts = p.last - p.first + 1;
-  // the first block may have begun with another pair
-  const float* first = a.part + (2LL * p.first + (p.first == c ? (half && st.begins < p.unit) : a.stretches[p.first].begins < p.unit)) * G * (D + 2);
-  auto part = [&](int x) { return x == 0 ? first : a.part + 2LL * (p.first + x) * G * (D + 2); };
+  const int parts = p.last - p.first + 1, size = part_floats(G, D);
+  auto part = [&](int x) { return a.part + (2LL * (p.first + x) + (x == 0 ? p.second : 0)) * size; };
+  const bool writes = cut && c == p.first + 1;
+  // four columns a thread, of the first parts
+  float4 column[kAhead];
+  if (writes && 4 * in_half < G * D) {
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) column[x] = *reinterpret_cast<const float4*>(part(min(x, parts - 1)) + 4 * in_half);
+  }
   if (cut) {
     for (int g = in_half >> 5; g < G; g += kHalf / 32) {
       float top = -FLT_MAX, sum = 0.f;
-      for (int x = lane; x < parts; x += 32) top = fmaxf(top, part(x)[G * D + 2 * g]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       for (int x = lane; x < parts; x += 32) {
         const float2 ml = *reinterpret_cast<const float2*>(part(x) + G * D + 2 * g);
-        const float f = exp2f(ml.x - top);
-        s_scale[half][x * G + g] = f;
-        sum += ml.y * f;
+        const float next = fmaxf(top, ml.x);
+        sum = sum * exp2f(top - next) + ml.y * exp2f(ml.x - next);
+        top = next;
+        s_scale[half][x * G + g] = ml.x;
       }
+      float most = top;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      sum *= exp2f(top - most);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) s_final[half][g] = make_float2(top, 1.f / sum);
+      if (lane == 0) s_final[half][g] = make_float2(most, 1.f / sum);
+      for (int x = lane; x < parts; x += 32) s_scale[half][x * G + g] = exp2f(s_scale[half][x * G + g] - most);
     }
   }
   __syncthreads();
-  if (cut && c == p.first + 1) {
-    for (int i = in_half; i < G * D; i += kHalf) {
+  if (writes) {
+    for (int i = 4 * in_half; i < G * D; i += 4 * kHalf) {
       const int g = i / D;
-      float v = 0.f;
-#pragma unroll 8
-      for (int x = 0; x < parts; ++x) v += part(x)[i] * s_scale[half][x * G + g];
-      a.out[static_cast<long long>(p.pair) * G * D + i] = from_f32<bf16>(v * s_final[half][g].y);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](const float4& p4, float f) {
+        v.x += p4.x * f;
+        v.y += p4.y * f;
+        v.z += p4.z * f;
+        v.w += p4.w * f;
+      };
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if (i > 4 * in_half) column[x] = *reinterpret_cast<const float4*>(part(min(x, parts - 1)) + i);
+        if (x < parts) add(column[x], s_scale[half][x * G + g]);
+      }
+#pragma unroll 4
+      for (int x = kAhead; x < parts; ++x) add(*reinterpret_cast<const float4*>(part(x) + i), s_scale[half][x * G + g]);
+      const float inv = s_final[half][g].y;
+      *reinterpret_cast<uint2*>(a.out + static_cast<long long>(p.pair) * G * D + i) =
+          make_uint2(bf_pack(v.x * inv, v.y * inv), bf_pack(v.z * inv, v.w * inv));
     }
   }
-  if (!a.scores) return;
-  for (; u < st.ends; u += kFinishThreads / 32) {
+  if (!tile) return;
+  while (true) {
     const int row = at.y + 2 * lane, rows = at.z;
     float* w = a.c.weights + static_cast<long long>(at.x) * a.c.width * a.c.page + row;
     const float2 old = row < rows ? *reinterpret_cast<const float2*>(w) : make_float2(0.f, 0.f);
@@ -820,17 +915,39 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args
     } else if (at.x == st.end[1].pair && st.end[1].first < st.end[1].last) {
       final = s_final[1];
     }
+    // the next tile is asked for before this one's numbers are needed
+    const bool more = u + kFinishThreads / 32 < st.ends;
+    const float* next_scores = scores + kFinishThreads / 32 * G * kTile;
+    int4 next_at = at;
+    float2 next[kAhead];
+    if (more) {
+      next_at = a.tile_rows[u + kFinishThreads / 32];
+#pragma unroll
+      for (int g = 0; g < kAhead; ++g) next[g] = *reinterpret_cast<const float2*>(next_scores + min(g, G - 1) * kTile);
+    }
     float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) {
+      if (g >= G) continue;
+      const float2 f = final[g];
+      s0 += exp2f(ahead[g].x - f.x) * f.y;
+      s1 += exp2f(ahead[g].y - f.x) * f.y;
+    }
 #pragma unroll 4
-    for (int g = 0; g < G; ++g) {
-      const float2 s = *reinterpret_cast<const float2*>(a.scores + (static_cast<long long>(u) * G + g) * kTile + 2 * lane), f = final[g];
+    for (int g = kAhead; g < G; ++g) {
+      const float2 s = *reinterpret_cast<const float2*>(scores + g * kTile), f = final[g];
       s0 += exp2f(s.x - f.x) * f.y;
       s1 += exp2f(s.y - f.x) * f.y;
     }
     // a new row's weight starts from 0
     if (row < rows) w[0] = (kStep && row == rows - 1 ? 0.f : old.x) + s0;
     if (row + 1 < rows) w[1] = (kStep && row + 1 == rows - 1 ? 0.f : old.y) + s1;
-    if (u + kFinishThreads / 32 < st.ends) at = a.tile_rows[u + kFinishThreads / 32];
+    if (!more) return;
+    u += kFinishThreads / 32;
+    scores = next_scores;
+    at = next_at;
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) ahead[g] = next[g];
   }
 }
 
@@ -865,7 +982,7 @@ Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
   l.tiles = (rows + kTile - 1) / kTile;
   if (!l.cluster) {
     take(sizeof(Stretch) * kMostBlocks);
-    l.part = take(sizeof(float) * kMostBlocks * 2 * G * (D + 2));
+    l.part = take(sizeof(float) * kMostBlocks * 2 * part_floats(G, D));
     l.tile_rows = weights ? take(sizeof(int4) * l.tiles * pairs) : 0;
     l.top_sum = weights ? take(sizeof(float2) * pairs * G) : 0;
   }
