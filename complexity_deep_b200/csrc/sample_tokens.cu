@@ -4,9 +4,9 @@
 //   index, i stays where the mass ahead of it is at most p times the mass that top-k has left;  min-p: w_i >= min_p;
 //   id = the first i, in the order of the vocabulary, with sum_{j <= i} w_j > u sum_j w_j over what stayed.
 //
-// The result is a whole number that hangs on where sums lie next to a border, so weights are good to 2^-32 of themselves and held as
-// multiples of 2^-44: sums of up to 2^18 of them are exact, and the same in any order. Nine products and sums in 32 bits and one of
-// whole numbers give such a weight (Row::mass); in 64-bit arithmetic it took 2.6 times as long (64 rows of 100 000: 94 us).
+// The result is a whole number that hangs on where sums lie next to a border, so weights are good to 2^-31 of themselves and held as
+// multiples of 2^-44: sums of up to 2^18 of them are exact, and the same in any order. Some thirty instructions on 32 bits give such a
+// weight (Row::mass); in 64-bit arithmetic it took 2.6 times as long.
 //
 // A cluster of blocks a row, which is read once and stays in their shared memory. A warp has a stretch of neighbouring tokens, its
 // lanes take 16 bytes of it in turn.
@@ -18,6 +18,7 @@
 // Where everything counts (no top-k, a large one, many equal values), the border of the top-k or of the nucleus is looked for by
 // histograms over equal steps of the value between the largest and the smallest one left: counts, or masses as three numbers of 15
 // bits, then the bin of the border alone, by pairs where it holds few values and in finer steps where it does not.
+#include <cfloat>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "elem.cuh"
@@ -29,7 +30,8 @@ namespace cdeep {
 namespace {
 
 constexpr int kList = 512;                 // entries compared pair by pair
-constexpr int kFew = 192;                  // the largest k that takes the bound
+constexpr int kFew = 256;                  // the largest k that takes the bound
+constexpr int kMany = 2048;                // tokens that a larger top-k leaves in a block, as a list
 constexpr int kMostBlocks = 8;             // of a row: the largest cluster that every device takes
 constexpr int kSliceBytes = 144 * 1024;    // of a row in a block: 2^18 numbers of 32 bits are eight blocks of 128 KB
 using u64 = unsigned long long;
@@ -87,7 +89,7 @@ template <int kThreads>
 struct Shared {
   static constexpr int kWarps = kThreads / 32, kBins = 2 * kThreads;
   u64 list[kList + 4], mass[kList + 4];    // tokens; their masses
-  u64 sorted[kList];
+  u64 sorted[kList], many[kMany];
   unsigned all_tops[kThreads + 4];
   unsigned powers[256];                    // 2^(j / 256 + 31)
   u64 sums[kWarps];
@@ -96,6 +98,7 @@ struct Shared {
   unsigned hist[3][kBins];
   unsigned tops[kThreads];
   unsigned high, low, tau, count, key;
+  unsigned ends[2];                        // keys of a bin
   unsigned counts[kMostBlocks];
   int bin;
 };
@@ -106,6 +109,7 @@ struct Row {
   Shared<kThreads>* s;
   const uint4* data;                       // this block's share of the row
   int begin, stretch;                      // its first token, tokens of a warp
+  int many = -1;
   int rank, blocks;
   uint32_t best;
   float top, rate, rate_low;               // 256 log2 e / T as two numbers
@@ -117,23 +121,41 @@ struct Row {
       __syncthreads();
     }
   }
-  // f(key, token index) for this thread's share; -inf and NaN are the keys up to kMinusInf
+  // This thread's share of the tokens, in the order of the vocabulary: warps have stretches, lanes 16 bytes of it in turn, or one
+  // entry of the list of tokens that top-k has left (many >= 0 of them in this block).
+  __device__ __forceinline__ int width() const { return many < 0 ? kVec : 1; }
+  __device__ __forceinline__ int from() const { return static_cast<int>(threadIdx.x >> 5) * stretch; }
+  __device__ __forceinline__ int to() const { return many < 0 ? from() + stretch : min(many, from() + stretch); }
+  // f(key, token index) for the tokens at place v; -inf and NaN are the keys up to kMinusInf
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    const int lane = threadIdx.x & 31, from = (threadIdx.x >> 5) * stretch;
-    for (int v = from + lane * kVec; v < from + stretch; v += 32 * kVec) vec(v, f);
-  }
-  template <typename F>
-  __device__ __forceinline__ void vec(int v, F f) const {
+  __device__ __forceinline__ void at(int v, F f) const {
+    if (many >= 0) {
+      const u64 t = s->many[v];
+      f(static_cast<uint32_t>(t >> 32), static_cast<int>(~static_cast<uint32_t>(t)));
+      return;
+    }
     const uint4 q = data[v / kVec];
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int e = 0; e < kVec; ++e) f(Key<T>::unpack(w, e), begin + v + e);
   }
-  // exp((x - max) / T) as a multiple of 2^-44, good to 2^-32 of itself: y = (x - max) 256 log2 e / T as a sum of two numbers, the
-  // whole part n of its 256ths from the table, 2^(f / 256) = 1 + q of the rest by a polynomial, q in 2^-31ths.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int w = width();
+    for (int v = from() + static_cast<int>(threadIdx.x & 31) * w; v < to(); v += 32 * w) at(v, f);
+  }
+  // f(places of the lanes' tokens) for the warp's steps: lanes beyond the end get a place that is not below to()
+  template <typename F>
+  __device__ __forceinline__ void steps(F f) const {
+    const int w = width();
+    for (int v = from(); v < to(); v += 32 * w) f(v + static_cast<int>(threadIdx.x & 31) * w);
+  }
+  // exp((x - max) / T) as a multiple of 2^-44, good to 2^-31 of itself: y = (x - max) 256 log2 e / T as a sum of two numbers, the
+  // whole part n of its 256ths from the table, 2^(f / 256) = 1 + q of the rest by a polynomial, q in 2^-31ths. The largest has exactly
+  // 1; an infinite one counts as the largest number that there is. What lies below 2^-45, and -inf, shift everything out; nobody asks
+  // for the mass of NaN.
   __device__ __forceinline__ u64 mass(uint32_t key) const {
-    const float x = Key<T>::value(key), d = x - top;
+    const float x = fminf(Key<T>::value(key), FLT_MAX), d = x - top;
     float rest = 0.f;
     if constexpr (sizeof(T) == 4) {                       // what the difference has lost (of bf16 numbers: nothing that counts)
       const float back = d - x;
@@ -142,15 +164,17 @@ struct Row {
     const float y = d * rate;
     const float low = fmaf(d, rate_low, fmaf(rest, rate, fmaf(d, rate, -y)));
     const float t = y + 12582912.f;                       // 1.5 2^23: rounds to a whole number, in the low bits
-    const int n = __float_as_int(t) - 0x4b400000;
+    const uint32_t n = __float_as_uint(t);                // 0x4b400000 + the whole part
     const float f = (y - (t - 12582912.f)) + low;
     const float q = f * fmaf(f, fmaf(f, 3.3083e-9f, 3.66556e-6f), 2.7076062e-3f);       // (ln 2 / 256)^i / i!
-    const int q31 = __float_as_int(q + 5.859375e-3f) - 0x3bc00000;                      // 1.5 2^-8
-    const u64 w = static_cast<u64>(s->powers[n & 255]) * (0x80000000u + q31);           // times 2^62
-    const int shift = (18 - (n >> 8)) & 63;
-    const u64 m = (w + (1ull << (shift - 1))) >> shift;
-    // at the largest exactly 1, also where that is infinite; below 2^-45, and at -inf, 0
-    return key == best ? kOne : y > -256.f * 45 ? m : 0;
+    const uint32_t one_q = __float_as_uint(q + 5.859375e-3f) + (0x80000000u - 0x3bc00000u);   // 1.5 2^-8; (1 + q) 2^31
+    const uint32_t w = __umulhi(s->powers[n & 255], one_q);                              // times 2^30
+    const uint32_t shift = 18 + 0x4b4000u - (n >> 8);     // of w 2^32
+    uint32_t hi, lo, far;
+    asm("shr.u32 %0, %1, %2;" : "=r"(hi) : "r"(w), "r"(shift));             // by 32 and more: 0
+    asm("shr.u32 %0, %1, %2;" : "=r"(far) : "r"(w), "r"(shift - 32));
+    asm("shf.r.clamp.b32 %0, 0, %1, %2;" : "=r"(lo) : "r"(w), "r"(shift));
+    return static_cast<u64>(hi) << 32 | (shift < 32 ? lo : far);
   }
 };
 
@@ -256,7 +280,6 @@ __device__ __forceinline__ u64 row_sum(const Row<T, kThreads>& r, u64 own) {
 // The r-th (from 0) of the tokens with this key, in the order of the vocabulary; all if there are no more than r.
 template <typename T, int kThreads>
 __device__ __forceinline__ int nth_equal(const Row<T, kThreads>& r, uint32_t key, u64 nth) {
-  constexpr int kVec = Row<T, kThreads>::kVec;
   Shared<kThreads>& s = *r.s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) s.found = ~0ull;
@@ -266,18 +289,17 @@ __device__ __forceinline__ int nth_equal(const Row<T, kThreads>& r, uint32_t key
   const u64 mine = s.sums[warp];
   u64 before = s.before + warp_sum(lane < warp ? s.sums[lane] : 0);
   if (before <= nth && nth < before + mine) {             // it lies in this warp's stretch
-    for (int v0 = warp * r.stretch; v0 < (warp + 1) * r.stretch; v0 += 32 * kVec) {
-      const int v = v0 + lane * kVec;
+    r.steps([&](int v) {
       u64 n = 0;
-      if (v < (warp + 1) * r.stretch) r.vec(v, [&](uint32_t k, int) { n += k == key; });
+      if (v < r.to()) r.at(v, [&](uint32_t k, int) { n += k == key; });
       const u64 upto = warp_upto(n);
       u64 at = before + upto - n;
       if (n > 0 && at <= nth && nth < at + n)
-        r.vec(v, [&](uint32_t k, int i) {
+        r.at(v, [&](uint32_t k, int i) {
           if (k == key && at++ == nth) s.found = i;
         });
       before += __shfl_sync(0xffffffffu, upto, 31);
-    }
+    });
   }
   r.sync();
   u64 found = s.found;
@@ -309,7 +331,7 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
     r.each([&](uint32_t k, int) {
       const int b = bin_of(k);
       const u64 m = kMass ? r.mass(k) : 1;
-      if (k < low || k > high) return;
+      if (k - low > high - low) return;
       if constexpr (kMass) {
         atomicAdd(&s.hist[0][b], static_cast<unsigned>(m & 0x7fff));
         atomicAdd(&s.hist[1][b], static_cast<unsigned>(m >> 15 & 0x7fff));
@@ -341,9 +363,25 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
     if (last == bin && last >= 0) s.before = before + (last & 1 ? held[0] : 0);
     __syncthreads();
     left -= s.before;
+    // the bin as a range of keys: bins fall as keys rise, so its ends are the last keys above it and up to it
+    if (tid < 64) {
+      const int least = bin + (tid < 32);                 // warp 0: the last key of a larger bin; warp 1: of this or a larger one
+      uint32_t a = low, b = high;
+      const bool any = bin_of(low) >= least;
+      while (any && a < b) {
+        const uint32_t step = (b - a) / 32 + 1, k = a + min((tid & 31) * step, b - a);
+        const unsigned yes = __ballot_sync(0xffffffffu, bin_of(k) >= least);
+        const uint32_t first = a + min((31 - __clz(yes)) * step, b - a);
+        b = first + min(step - 1, b - first);
+        a = first;
+      }
+      if ((tid & 31) == 0) s.ends[tid >> 5] = tid < 32 ? (any ? a + 1 : low) : a;
+    }
+    __syncthreads();
+    const uint32_t bottom = s.ends[0], span = s.ends[1] - bottom;
     unsigned hi = 0, lo = 0xffffffffu;
     const unsigned n = collect(r, [&](uint32_t k, int) {
-      if (bin_of(k) != bin || k < low || k > high) return false;
+      if (k - bottom > span) return false;
       hi = max(hi, k);
       lo = min(lo, k);
       return true;
@@ -396,6 +434,43 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
     left = __umul64hi(left, row_sum(r, own) * m);
   }
   return token(high, nth_equal(r, high, m > 0 ? left / m : ~0ull));
+}
+
+// Where the block has few enough tokens from key `from` on, a list of them takes its share's place, in order.
+template <typename T, int kThreads>
+__device__ __forceinline__ void list_from(Row<T, kThreads>& r, uint32_t from) {
+  Shared<kThreads>& s = *r.s;
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int own = 0;
+  r.each([&](uint32_t k, int) { own += k >= from; });
+  own = __reduce_add_sync(0xffffffffu, own);
+  __syncthreads();
+  if (lane == 0) s.sums[warp] = own;
+  __syncthreads();
+  const int other = lane < kWarps ? static_cast<int>(s.sums[lane]) : 0;
+  const int all = __reduce_add_sync(0xffffffffu, other);
+  int before = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0);
+  if (all > kMany) return;
+  r.steps([&](int v) {
+    int n = 0;
+    if (v < r.to()) r.at(v, [&](uint32_t k, int) { n += k >= from; });
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    int at = before + upto - n;
+    if (n > 0)
+      r.at(v, [&](uint32_t k, int i) {
+        if (k >= from) s.many[at++] = token(k, i);
+      });
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  });
+  r.many = all;
+  r.stretch = (all + kWarps - 1) / kWarps;
+  __syncthreads();
 }
 
 template <typename T, int kThreads>
@@ -463,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   // the largest lane maxima of every warp
   const int warps = min(r.blocks * kWarps, (V + stretch - 1) / stretch);     // that have tokens
   const int draws = (2 * top_k + warps - 1) / warps;
-  const bool few = top_k > 0 && top_k < V && top_k <= kFew && draws <= 32;
+  const bool few = top_k > 0 && top_k < V && top_k <= kFew && draws <= 32 && warps * draws <= kThreads;
   if (few) {
     uint32_t m = high;
     for (int d = 0; d < draws; ++d) {
@@ -505,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   r.sync();
   const uint32_t reach = max(s.tau, Key<T>::kMinusInf + 1);
   r.best = best;
-  r.top = Key<T>::value(best);
+  r.top = fminf(Key<T>::value(best), FLT_MAX);
   const double rate = 369.32993046757462 / static_cast<double>(temperature);   // 256 log2 e
   r.rate = static_cast<float>(rate);
   r.rate_low = static_cast<float>(rate - static_cast<double>(r.rate));
@@ -582,12 +657,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
     }
     return;
   }
-  if (top_k > 0 && top_k < V) from = max(from, static_cast<uint32_t>(border<false>(r, least, best, static_cast<u64>(top_k - 1)) >> 32));
+  if (top_k > 0 && top_k < V) {
+    from = max(from, static_cast<uint32_t>(border<false>(r, least, best, static_cast<u64>(top_k - 1)) >> 32));
+    list_from(r, from);
+  }
   u64 last = token(from, 0x7fffffff);                     // the last token that stays
   if (top_p < 1.f) last = border<true>(r, max(from, least), best, share);
+  const uint32_t last_key = last >> 32;
+  const int last_equal = static_cast<int>(~static_cast<uint32_t>(last));
   auto held = [&](uint32_t k, int i) -> u64 {
     const u64 w = r.mass(k);
-    return token(k, i) < last || w < least_mass ? 0 : w;
+    return k < last_key || (k == last_key && i > last_equal) || w < least_mass ? 0 : w;
   };
   u64 own = 0;
   r.each([&](uint32_t k, int i) { own += held(k, i); });
@@ -595,14 +675,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   const u64 mine = s.sums[warp];
   u64 before = s.before + warp_sum(lane < warp ? s.sums[lane] : 0);
   if (before <= target && target < before + mine) {       // in this warp's stretch
-    for (int v0 = warp * stretch; v0 < (warp + 1) * stretch; v0 += 32 * kVec) {
-      const int v = v0 + lane * kVec;
+    r.steps([&](int v) {
       u64 w = 0;
-      if (v < (warp + 1) * stretch) r.vec(v, [&](uint32_t k, int i) { w += held(k, i); });
+      if (v < r.to()) r.at(v, [&](uint32_t k, int i) { w += held(k, i); });
       const u64 upto = warp_upto(w);
       u64 at = before + upto - w;
       if (w > 0 && at <= target && target < at + w)
-        r.vec(v, [&](uint32_t k, int i) {
+        r.at(v, [&](uint32_t k, int i) {
           const u64 e = held(k, i);
           if (e > 0 && at <= target && target < at + e) {
             ids[b] = i;
@@ -611,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
           at += e;
         });
       before += __shfl_sync(0xffffffffu, upto, 31);
-    }
+    });
   }
 }
 

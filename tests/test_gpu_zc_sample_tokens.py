@@ -49,6 +49,18 @@ def test_vocabularies(V):
             _check(x, u, *rules)
 
 
+@pytest.mark.parametrize("k", [192, 193, 200, 255, 256, 257, 511, 512, 513, 2047, 2048, 2049, 4999, 8191, 8192])
+def test_sizes_of_top_k(k):
+    """Around the largest k that takes the bound, the lists' sizes and the vocabulary."""
+    for V in (8192, 50000):
+        for dtype in (torch.bfloat16, torch.float32):
+            x, u = _inputs(3, V, dtype, V + k)
+            _check(x, u, 1.0, k, 0.9, 0.0)
+            _check(x, u, 1.5, k, 1.0, 0.01)
+    x = torch.randint(0, 50, (3, 9000), generator=torch.Generator().manual_seed(k)).to(torch.bfloat16)   # ties at every border
+    _check(x, torch.rand(3, generator=torch.Generator().manual_seed(k)), 8.0, k, 0.8, 0.0)
+
+
 def test_largest_vocabulary():
     x, u = _inputs(2, 1 << 18, torch.float32, 1)
     _check(x, u, 1.0, 0, 0.9, 0.0)
