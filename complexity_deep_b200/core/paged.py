@@ -79,7 +79,7 @@ class PagedKVCache:
         del self._pages[slot][count:]
 
     def _send(self) -> None:
-        self.table.copy_(self._table)
+        self.table.copy_(self._table, non_blocking=True)     # from pageable memory: the host's copy is free when the call returns
 
     def add(self, past_key_values, row: int = 0) -> int:
         """Takes over the cache of sequence `row` of a prompt (list of (k, v) [B, kv heads, P, D]) and returns the slot."""

@@ -1034,6 +1034,7 @@ static int paged_attention(const cd_paged* c, const cd_paged_step* step, const v
   if (st == CD_OK) st = paged_shape_ok(hq, hkv, D, c->page);
   if (st != CD_OK) return st;
   if (!q || !out || !aligned16(q) || !aligned16(out) || (q_stride & 7) || q_stride < 0) return CD_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(c->weights) & 7) return CD_ERR_INVALID;
   const size_t need = paged_attention_workspace_bytes(B, hq, hkv, D, c->page, c->width, c->weights != nullptr);
   if (need && (!ws || !aligned16(ws) || ws_bytes < need)) return CD_ERR_INVALID;
   if ((static_cast<long long>(c->width) * c->page + 63) / 64 * B * hkv > 0x7fffffffLL) return CD_ERR_UNSUPPORTED;   // tiles are counted in 32 bits
@@ -1081,7 +1082,7 @@ int cd_evict_rows(const cd_paged* c, const cd_evict* e, int layers, long long st
 
 int cd_sample_tokens(const void* logits, int fp32, long long ld, int B, int V, const cd_sample* p, int64_t* ids, float* probs,
                      void* stream) {
-  if (!logits || !p || !p->uniform || !ids || !probs || B < 1 || V < 1 || ld < V) return CD_ERR_INVALID;
+  if (!logits || !p || !p->uniform || !ids || !probs || B < 1 || V < 1 || ld < 0) return CD_ERR_INVALID;
   if (V > (1 << 18)) return CD_ERR_UNSUPPORTED;                    // masses are sums of 2^18 numbers up to 2^44
   const cudaError_t e = launch_sample_tokens(logits, fp32 ? 1 : 0, ld, B, V, *p, ids, probs, as_stream(stream));
   return e == cudaSuccess ? CD_OK : cuda_fail(e, "sample tokens launch");

@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kSmallThreads ? 7 : 1) e
   griddep_launch_dependents();
   const int pair = blockIdx.x / a.blocks, rank = blockIdx.x - pair * a.blocks;
   const int h = pair % a.hkv, b = pair / a.hkv % a.B, layer = pair / (a.hkv * a.B);
-  const int keep = a.e.keep, n = min(a.c.lengths[b], a.rows);
+  const int keep = a.e.keep, n = a.c.lengths[b];
   const long long base = static_cast<long long>(pair) * a.rows;
   const float* w = a.c.weights + base;
   const int* pos = a.e.row_positions + base;
@@ -76,7 +76,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == kSmallThreads ? 7 : 1) e
   int* pos_out = a.e.row_positions_out + base;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool in_place = w_out == w;
-  if (n <= keep) {                        // the same for all blocks of the pair
+  if (n > a.rows) {                       // the same for all blocks of the pair, as below
+    if (threadIdx.x == 0) atomicMax(a.status, kStatusBounds);
+    return;
+  }
+  if (n <= keep) {
     if (!in_place)
       for (int i = rank * kThreads + tid; i < n; i += a.blocks * kThreads) w_out[i] = w[i], pos_out[i] = pos[i];
     return;

@@ -474,7 +474,7 @@ __device__ __forceinline__ void list_from(Row<T, kThreads>& r, uint32_t from) {
 }
 
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kernel(const T* logits, long long ld, int V, int slice, int stretch, cd_sample p,
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kernel(const T* logits, long long ld, int V, int blocks, int slice, int stretch, cd_sample p,
                                                                  long long* ids, float* probs) {
   constexpr int kVec = Row<T, kThreads>::kVec, kWarps = kThreads / 32;
   extern __shared__ uint4 s_dyn[];
@@ -489,11 +489,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   Row<T, kThreads> r;
   r.s = &s;
   r.data = s_data;
-  r.blocks = gridDim.x;
-  r.rank = blockIdx.x;
+  r.blocks = blocks;
+  r.rank = blockIdx.x % blocks;
   r.begin = r.rank * slice;
   r.stretch = stretch;
-  const int b = blockIdx.y, length = max(0, min(slice, V - r.begin));
+  const int b = blockIdx.x / blocks, length = max(0, min(slice, V - r.begin));
   const T* x = logits + b * ld + r.begin;
   const float temperature = p.temperatures ? p.temperatures[b] : p.temperature;
   const float top_p = p.top_ps ? p.top_ps[b] : p.top_p;
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   const uint32_t reach = max(s.tau, Key<T>::kMinusInf + 1);
   r.best = best;
   r.top = fminf(Key<T>::value(best), FLT_MAX);
-  const double rate = 369.32993046757462 / static_cast<double>(temperature);   // 256 log2 e
+  const double rate = fmin(369.32993046757462 / static_cast<double>(temperature), 1e38);   // 256 log2 e, and finite: 0 times it is 0
   r.rate = static_cast<float>(rate);
   r.rate_low = static_cast<float>(rate - static_cast<double>(r.rate));
 
@@ -712,7 +712,7 @@ cudaError_t launch_blocks(int blocks, const T* logits, long long ld, int B, int 
   const cudaError_t e = allow_smem<kKernel>(bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks, B);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks) * B);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
@@ -724,7 +724,7 @@ cudaError_t launch_blocks(int blocks, const T* logits, long long ld, int B, int 
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = blocks > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kKernel, logits, ld, V, slice, stretch, p, ids, probs);
+  return cudaLaunchKernelEx(&cfg, kKernel, logits, ld, V, blocks, slice, stretch, p, ids, probs);
 }
 
 // As many blocks a row as its size asks for, and more while there is an SM for each and 4 096 tokens. us, 1 / 2 / 4 / 8 blocks of 512

@@ -1450,6 +1450,8 @@ def _evict_workspace(device: int, *sizes) -> int:
 def _attend_paged(step, c: _lib.Paged, q: torch.Tensor, batch: int, hq: int, hkv: int, D: int, device: int) -> torch.Tensor:
     lib = _lib.load()
     out = q.new_empty(batch, hq * D)
+    if not batch:
+        return out
     n = _paged_workspace(device, batch, hq, hkv, D, c.page, c.width, 0 if c.weights is None else 1)
     ws = q.new_empty(n // 2) if n else None
     with _Span("paged_attention", 2):
@@ -1479,7 +1481,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     buffer will do), pages [pages, hkv, page, D] of any strides, block_table int32 [B, width] (row r of a sequence is in page
     ``block_table[b, r // page]``), lengths int32 [B] on the device (0 or less: the output row is zeros).  `weights` (fp32
     [B, hkv, width * page]): every row's softmax weight, summed over the query heads of its KV head, is added there.
-    Returns [B, hq * D].  A page outside the pool raises in ``status_fetch``."""
+    Returns [B, hq * D].  Rows behind a sequence's end may hold anything; a key or value of its own that is not finite makes its
+    head (its column) NaN.  A page outside the pool raises in ``status_fetch``."""
     device = _here(q, "q")
     _heads(k_pages, hq, hkv, head_dim)
     if q.dtype is not BF16 or q.dim() != 2 or q.stride(1) != 1 or q.shape[1] < hq * head_dim or q.stride(0) % 8 or q.data_ptr() & 15:
@@ -1555,6 +1558,8 @@ def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
                    _on(row_positions, "row_positions", torch.int32, device, shape),
                    _on(weights_out, "weights_out", torch.float32, device, shape),
                    _on(row_positions_out, "row_positions_out", torch.int32, device, shape), keep, recent)
+    if not B:
+        return
     lib = _lib.load()
     n = _evict_workspace(device, layers, B, hkv, c.page, c.width, keep)
     ws = k_pages.new_empty(n // 2) if n else None
@@ -1570,7 +1575,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     values at least the k-th largest (ties stay, as in ``sample_next``), top_p what has at most top_p of the remaining mass ahead
     of it in descending order (ties: lowest index first), min_p what has w >= min_p; the id is the first i, in the order of the
     vocabulary, with sum_{j <= i} w_j > uniform * sum_j w_j.  Every rule is a number, or a tensor with one entry per row (fp32,
-    top_k int32).  temperature 0 takes the first largest value; top_k 0, top_p 1 and min_p 0 are off.  A NaN is never drawn; a row
+    top_k int32).  temperature 0 takes the first largest value; top_k 0, top_p 1 and min_p 0 are off.  A NaN is never drawn, +inf counts as the largest number; a row
     without a value above -inf gives id 0 with probability 0."""
     device = _here(logits, "logits")
     if logits.dtype not in (BF16, torch.float32) or logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:

@@ -678,7 +678,7 @@ typedef struct cd_paged {
   const int32_t* table;     /* [B, width], rows table_stride apart */
   long long table_stride;
   const int32_t* lengths;   /* [B] cached rows */
-  float* weights;           /* [B, kv heads, width * page] accumulated attention weights, or NULL */
+  float* weights;           /* [B, kv heads, width * page] accumulated attention weights (on an 8-byte boundary), or NULL */
   int pages, page, width;   /* page: 16, 32, 64, 128 or 256 rows */
 } cd_paged;
 
@@ -696,7 +696,8 @@ typedef struct cd_paged_step {
 
 /* One query per sequence over its lengths[b] rows (none: zeros; below 0: the same):
  *   out[b, h] = softmax(scale q[b, h] . K_b^T) V_b;  weights[b, h / G, r] += sum over the G heads of p[r]
- * Sequences may share pages.  D is 64 or 128, G = hq / hkv <= 16; q rows q_stride_b elements apart (a
+ * Sequences may share pages.  Rows behind a sequence's end are never used, whatever they hold; a key or value of
+ * its own that is not finite makes its head (its column) NaN.  D is 64 or 128, G = hq / hkv <= 16; q rows q_stride_b elements apart (a
  * multiple of 8).  ws: cd_paged_attention_workspace_bytes(...) bytes, NULL where that is 0. */
 size_t cd_paged_attention_workspace_bytes(int B, int hq, int hkv, int D, int page, int width, int weights);
 int cd_paged_attention(const cd_paged* h_cache, const void* q, long long q_stride_b, float scale, int B,
@@ -728,12 +729,13 @@ int cd_evict_rows(const cd_paged* h_cache, const cd_evict* h_evict, int layers, 
                   int D, void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------ sampling -----------------
- * The next token of every row of logits [B, V] (bf16 or fp32, rows ld elements apart), from given uniform
+ * The next token of every row of logits [B, V] (bf16 or fp32, rows ld >= 0 elements apart), from given uniform
  * numbers.  With w = exp((x - max) / temperature): top-k keeps values at least the k-th largest (ties stay),
  * top-p what has, in descending order (ties: lowest index first), at most top_p of the mass that top-k has left
  * ahead of it, min-p what has w >= min_p; the id is the first i with sum_{j <= i} w_j > uniform sum_j w_j.
  * probs: w_id / sum.  temperature <= 0: the first largest value.  top_k <= 0, top_p >= 1, min_p <= 0: off.  A
- * NaN is never drawn; a row without a value above -inf gives id 0 and probability 0.  V <= 2^18.  Replaces
+ * NaN is never drawn, +inf counts as the largest number; a row without a value above -inf gives id 0 and
+ * probability 0.  V <= 2^18.  Replaces
  * complexity_deep/models/modeling.py:256-296. */
 typedef struct cd_sample {
   const float* uniform;         /* [B] in [0, 1) */

@@ -212,6 +212,39 @@ def test_no_room_and_bad_tables():
     ops.status_fetch()
 
 
+def test_refusals():
+    from complexity_deep_b200 import ops
+    k, v, table = (t.cuda() for t in cases.make_cache([40, 40], 2, 64, 16, 1, room=1, rest=0.0))
+    q, n = torch.zeros(2, 8 * 64, dtype=BF, device="cuda"), torch.tensor([40, 40], dtype=torch.int32, device="cuda")
+    cos, sin = (t.cuda() for t in cases.tables(64, 64))
+    rows = table.shape[1] * 16
+    w = torch.zeros(2, 2, rows, device="cuda")
+    good = dict(q=q, k_pages=k, v_pages=v, block_table=table, lengths=n, hq=4, hkv=2, head_dim=64)
+    ops.paged_attention(**good)
+    odd = torch.zeros(2 * 2 * rows + 1, device="cuda")[1:].view(2, 2, rows)              # not on an 8-byte boundary
+    for bad in (dict(q=q.float()), dict(q=q[:, :255]), dict(q=q[:, 1:]), dict(k_pages=k.float()), dict(k_pages=k[:, :1]), dict(v_pages=v[:3]),
+                dict(k_pages=k.transpose(2, 3)), dict(block_table=table.long()), dict(block_table=table[:1]), dict(lengths=n.long()),
+                dict(lengths=n[:1]), dict(lengths=n.cpu()), dict(block_table=table.cpu()), dict(hq=3), dict(hq=34), dict(head_dim=32),
+                dict(weights=w[:, :1]), dict(weights=w.double()), dict(weights=odd), dict(k_pages=k[:, :, :12], v_pages=v[:, :, :12])):
+        with pytest.raises(Exception) as e:
+            ops.paged_attention(**{**good, **bad})
+        assert isinstance(e.value, RuntimeError), bad
+    step = dict(qkv=q, q_w=None, k_w=None, cos=cos, sin=sin, eps=1e-6, hq=4, hkv=2, head_dim=64, k_pages=k, v_pages=v, block_table=table,
+                lengths=n, positions=n)
+    ops.paged_step_attention(**step)
+    one = torch.ones(64, dtype=BF, device="cuda")
+    for bad in (dict(qkv=q[:, :256]), dict(q_w=one), dict(k_w=one), dict(q_w=one[:32], k_w=one), dict(cos=cos[:, :32]), dict(sin=sin[:9]),
+                dict(cos=cos.double()), dict(positions=n.long()), dict(row_positions=w)):
+        with pytest.raises(RuntimeError):
+            ops.paged_step_attention(**{**step, **bad})
+    assert ops.paged_attention(q[:0], k, v, table[:0], n[:0], 4, 2, 64).shape == (0, 256)
+    # tables and weights off their boundaries are taken all the same
+    shifted = torch.empty(64 * 64 + 1, device="cuda")[1:].view(64, 64).copy_(cos)
+    w1 = torch.ones(65, dtype=BF, device="cuda")[1:]
+    a = ops.paged_step_attention(**{**step, "q_w": one, "k_w": one})
+    assert torch.equal(a, ops.paged_step_attention(**{**step, "cos": shifted, "q_w": w1, "k_w": w1}))
+
+
 def test_captured_and_streams():
     """A captured step follows lengths that change between replays; two graphs and an eager call share nothing."""
     from complexity_deep_b200 import ops

@@ -126,3 +126,17 @@ def test_bad_page_is_skipped():
     with pytest.raises(_lib.CdeepError):
         ops.status_fetch()
     ops.status_fetch()
+
+
+def test_length_beyond_the_table_is_refused():
+    from complexity_deep_b200 import ops, _lib
+    k, v, table = cases.make_cache([64, 64], 1, 64, 16, 1, rest=0.0)
+    w, pos = torch.rand(2, 1, 64).cuda(), torch.zeros(2, 1, 64, dtype=torch.int32).cuda()
+    before, n, kd = w.clone(), torch.tensor([65, 40], dtype=torch.int32).cuda(), k.cuda()
+    ops.evict_rows_(kd, v.cuda(), table.cuda(), n, n, w, pos, 16, 0)
+    with pytest.raises(_lib.CdeepError):
+        ops.status_fetch()
+    assert torch.equal(w[0], before[0]) and not torch.equal(w[1], before[1])
+    mine = table[0].long()
+    assert torch.equal(kd[mine.cuda()].cpu(), k[mine])
+    assert ops.evict_rows_(kd, kd, table[:0].cuda(), n[:0], n[:0], w[:0], pos[:0], 16, 0) is None

@@ -116,6 +116,37 @@ def test_infinities_and_nan():
     assert ids.tolist() == [0, 0] and probs.tolist() == [0.0, 0.0]
 
 
+def test_odd_rules_and_strides():
+    """Rules at the ends of their ranges and beyond, given numbers outside [0, 1), one row of logits for many draws."""
+    from complexity_deep_b200 import ops
+    nan, inf = float("nan"), float("inf")
+    x, u = _inputs(1, 700, torch.float32, 4)
+    many = torch.linspace(0, 0.999, 300)
+    _check(x.expand(300, -1), many, 0.7, 30, 0.9, 0.0)
+    assert ops.sample_tokens(x.cuda().expand(300, -1), many.cuda(), 0.7, 30, 0.9)[0].shape == (300,)
+    best = int(x.argmax())
+    for t in (0.0, -1.0, nan, 1e-30, 1e-37, 1e-40):                        # greedy, or so cold that only the largest has a weight
+        ids, probs = ops.sample_tokens(x.cuda(), u.cuda(), t, 0, 0.9)
+        assert ids.tolist() == [best] and probs.tolist() == [1.0], t
+    want = ops.sample_tokens(x.cuda(), u.cuda())
+    for rules in ((1.0, -3, 1.0, 0.0), (1.0, 700, 1.0, 0.0), (1.0, 10 ** 9, 2.0, -1.0), (1.0, 0, nan, nan), (1.0, 0, inf, 0.0)):
+        assert torch.equal(ops.sample_tokens(x.cuda(), u.cuda(), *rules)[0], want[0]), rules
+    assert int(ops.sample_tokens(x.cuda(), u.cuda(), inf)[0]) == int(float(u) * 700)     # all weigh the same
+    ends = ops.sample_tokens(x.cuda().expand(5, -1), torch.tensor([-1.0, nan, 0.0, 1.0, 7.0]).cuda())[0].tolist()
+    assert ends[0] == ends[1] == ends[2] == 0 and ends[3] == ends[4] == 699
+    for p, m in ((0.0, 0.0), (-1.0, 0.0), (1.0, 1.0), (1.0, 5.0)):         # the largest alone
+        assert ops.sample_tokens(x.cuda(), u.cuda(), 1.0, 0, p, m)[0].tolist() == [best]
+
+
+def test_more_rows_than_a_grid_is_high():
+    from complexity_deep_b200 import ops
+    x = torch.zeros(70000, 8, device="cuda")
+    x[:, 3] = 50.0
+    x[69999, 3], x[69999, 5] = 0.0, 50.0
+    ids, _ = ops.sample_tokens(x, torch.full((70000,), 0.5, device="cuda"))
+    assert bool((ids[:-1] == 3).all()) and int(ids[-1]) == 5
+
+
 def test_captured_and_empty():
     from complexity_deep_b200 import ops
     x, u = (t.cuda() for t in _inputs(3, 4000, torch.bfloat16, 8))

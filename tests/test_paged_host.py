@@ -45,7 +45,7 @@ def test_workspaces():
     n = lib.cd_paged_attention_workspace_bytes(2, 4, 2, 64, 16, 4, 1)
     assert n >= 2 * 4 * 64 * 4
     assert _attend(_cache(weights=A)) == INVALID and _attend(_cache(weights=A), ws=A, n=n - 1) == INVALID
-    assert _attend(_cache(weights=A), ws=A + 4, n=n) == INVALID
+    assert _attend(_cache(weights=A), ws=A + 4, n=n) == INVALID and _attend(_cache(weights=A + 4), ws=A, n=n) == INVALID
     assert lib.cd_paged_attention_workspace_bytes(2, 4, 2, 96, 16, 4, 1) == 0
     assert lib.cd_evict_rows_workspace_bytes(1, 2, 2, 16, 4, 0) == 0
 
@@ -83,7 +83,7 @@ def test_sample_arguments():
         r = _lib.Sample(uniform=uniform, temperature=1.0, top_p=1.0)
         return lib.cd_sample_tokens(logits, 0, ld, B, V, ctypes.byref(r), ids, probs, None)
 
-    for change in (dict(logits=None), dict(uniform=None), dict(ids=None), dict(probs=None), dict(B=0), dict(V=0), dict(ld=99)):
+    for change in (dict(logits=None), dict(uniform=None), dict(ids=None), dict(probs=None), dict(B=0), dict(V=0), dict(ld=-1)):
         assert call(**change) == INVALID
     assert call(V=(1 << 18) + 1, ld=1 << 19) == UNSUPPORTED
     assert lib.cd_sample_tokens(A, 0, 100, 2, 100, None, A, A, None) == INVALID
