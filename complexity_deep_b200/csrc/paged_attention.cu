@@ -42,7 +42,7 @@ constexpr int kThreads = 32 * (kWarps + 2);
 constexpr int kSlots = kWarps / 2;        // in which warps hand over their sums
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMostCluster = 8;           // blocks of a pair
-constexpr int kClusterTiles = 8;          // tiles of a block, up to which pairs have clusters
+constexpr int kClusterTiles = 16;         // tiles of a block, up to which pairs have clusters
 
 __host__ __device__ constexpr int stage_bytes(int D) { return 2 * kTile * D * 2; }
 // floats of a lane that a warp hands over: its columns of each head it holds
@@ -957,11 +957,18 @@ int sm_count() {
   return n;
 }
 
-// Blocks of a pair where short caches take clusters, else 0.
-int cluster_of(long long pairs, long long tiles) {
+// Blocks of a pair where short caches take clusters, else 0: as many as give every block an SM to itself, twice as many where they
+// would have more than eight tiles and two fit an SM; up to 16 tiles a block. us, cold L2, events included, line / clusters of 1 / 2 / 4 / 8,
+// 8 heads of 2 x 128: 1 x 512 rows 15 / 16 / 13 / 12 / 12, 1 x 4 096 26 / 55 / 33 / 23 / 16, 4 x 1 024 20 / 21 / 16 / 14 / 16, 4 x 4 096
+// 30 / 55 / 35 / 27 / 27, 8 x 512 18 / 16 / 14 / 16 / 23, 8 x 2 048 30 / 33 / 27 / 25 / 33, 16 x 1 024 30 / 25 / 25 / 31, 16 x 2 048
+// 42 / 39 / 39 / 43, 32 x 256 22 / 19 / 24, 32 x 1 024 42 / 37 / 43, 64 x 128 22 / 23, 64 x 512 42 / 41; with weights, lengths between a
+// half and all: 8 x 1 024 24 / 27 / 23 / 21 / 27, 32 x 1 024 40 / 39 / 45.
+int cluster_of(long long pairs, long long tiles, int fit) {
+  const long long sms = sm_count();
   int blocks = 1;
-  while (blocks < kMostCluster && 2 * blocks * pairs <= 2LL * sm_count() && 2 * blocks <= tiles) blocks *= 2;
-  return blocks * pairs <= 2LL * sm_count() && (tiles + blocks - 1) / blocks <= kClusterTiles ? blocks : 0;
+  while (blocks < kMostCluster && 2 * blocks * pairs <= sms && 2 * blocks <= tiles) blocks *= 2;
+  if (blocks < kMostCluster && 2 * blocks * pairs <= fit * sms && tiles > kClusterTiles / 2 * blocks) blocks *= 2;
+  return blocks * pairs <= fit * sms && (tiles + blocks - 1) / blocks <= kClusterTiles ? blocks : 0;
 }
 
 // Where things lie in the workspace.
@@ -972,7 +979,7 @@ struct Layout {
 };
 Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
   Layout l = {};
-  l.cluster = cluster_of(static_cast<long long>(B) * hkv, (static_cast<long long>(width) * page + kTile - 1) / kTile);
+  l.cluster = cluster_of(static_cast<long long>(B) * hkv, (static_cast<long long>(width) * page + kTile - 1) / kTile, blocks_per_sm(D, G > 8));
   auto take = [&](size_t n) {
     const size_t at = l.bytes;
     l.bytes += (n + 255) / 256 * 256;

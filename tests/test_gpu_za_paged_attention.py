@@ -62,6 +62,14 @@ def test_long_and_many():
     _attend([-1, 9, -1], 2, 2, 64, 16, seed=8, weights=True)
 
 
+@pytest.mark.parametrize("G,D", [(1, 128), (3, 64), (8, 128), (9, 64), (16, 128), (16, 64)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_line_of_tiles(G, D, weights):
+    """More tiles than clusters take: pairs cut between many blocks, several pairs a block, sequences without rows in between."""
+    _attend([20000, 1, 0, 700], 2, G, D, 64, seed=G, weights=weights)
+    _attend([0] + [(97 * i) % 260 for i in range(130)] + [0], 3, G, D, 16, seed=G + 1, weights=weights, order="rows")
+
+
 def test_strides_and_shared_pages():
     """Pools that are every other page and a part of the heads of larger ones, a table that is a part of a wider one, two
     sequences that share their first pages."""
@@ -180,6 +188,12 @@ def test_step_sizes(norm):
     _step([300], 4, 3, 64, 16, norm=norm)
     _step([6000, 3], 8, 2, 128, 64, norm=norm, weights=True)
     _step([(53 * i) % 400 - 1 for i in range(40)], 8, 2, 128, 64, norm=norm, weights=True)
+
+
+@pytest.mark.parametrize("G,D", [(2, 64), (4, 128), (12, 64), (16, 128)])
+def test_step_on_a_line_of_tiles(G, D):
+    _step([20000, -1, 3, 639, 640], 2, G, D, 64, seed=G, weights=True)
+    _step([(97 * i) % 260 - 1 for i in range(130)], 3, G, D, 16, seed=G + 1, weights=True, order="rows")
 
 
 def test_no_room_and_bad_tables():
