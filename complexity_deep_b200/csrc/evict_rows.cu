@@ -60,6 +60,7 @@ __device__ __forceinline__ int warps_before(int v, int* s, int& all) {
 template <int kThreads, bool kHeld>
 __global__ void __launch_bounds__(kThreads, kThreads == kSmallThreads ? 7 : 1) evict_rows_kernel(const Args a) {
   constexpr int kWarps = kThreads / 32, kOwn = kBins / kThreads;
+  static_assert(kOwn < 4 || kOwn % 8 == 0, "a thread's bins are read four at a time, also of the 1 024 of the last histogram");
   extern __shared__ __align__(16) unsigned s_dyn[];
   __shared__ int s_warps[kWarps];
   __shared__ unsigned s_digit, s_left, s_equal;
