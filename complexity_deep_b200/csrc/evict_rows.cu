@@ -287,12 +287,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == kSmallThreads ? 7 : 1) e
   }
 }
 
-int sm_count() {
-  int device = 0, n = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 148;
-  return n;
-}
-
 template <int kThreads, bool kHeld>
 cudaError_t launch_one(const Args& a, int pairs, cudaStream_t stream) {
   constexpr auto kKernel = evict_rows_kernel<kThreads, kHeld>;
@@ -319,7 +313,7 @@ cudaError_t launch_one(const Args& a, int pairs, cudaStream_t stream) {
 int blocks_of(long long pairs, int rows, int keep) {
   const int most = rows - keep < keep ? rows - keep : keep;
   int blocks = 1;
-  while (blocks < kMostBlocks && 2 * blocks * pairs <= sm_count() && most >= 256 * blocks) blocks *= 2;
+  while (blocks < kMostBlocks && 2 * blocks * pairs <= current_sm_count() && most >= 256 * blocks) blocks *= 2;
   return blocks;
 }
 

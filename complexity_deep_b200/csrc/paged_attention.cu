@@ -951,12 +951,6 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args
   }
 }
 
-int sm_count() {
-  int device = 0, n = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 148;
-  return n;
-}
-
 // Blocks of a pair where short caches take clusters, else 0: as many as give every block an SM to itself, twice as many where they
 // would have more than eight tiles and two fit an SM; up to 16 tiles a block. us, cold L2, events included, line / clusters of 1 / 2 / 4 / 8,
 // 8 heads of 2 x 128: 1 x 512 rows 15 / 16 / 13 / 12 / 12, 1 x 4 096 26 / 55 / 33 / 23 / 16, 4 x 1 024 20 / 21 / 16 / 14 / 16, 4 x 4 096
@@ -964,7 +958,7 @@ int sm_count() {
 // 42 / 39 / 39 / 43, 32 x 256 22 / 19 / 24, 32 x 1 024 42 / 37 / 43, 64 x 128 22 / 23, 64 x 512 42 / 41; with weights, lengths between a
 // half and all: 8 x 1 024 24 / 27 / 23 / 21 / 27, 32 x 1 024 40 / 39 / 45.
 int cluster_of(long long pairs, long long tiles, int fit) {
-  const long long sms = sm_count();
+  const long long sms = current_sm_count();
   int blocks = 1;
   while (blocks < kMostCluster && 2 * blocks * pairs <= sms && 2 * blocks <= tiles) blocks *= 2;
   if (blocks < kMostCluster && 2 * blocks * pairs <= fit * sms && tiles > kClusterTiles / 2 * blocks) blocks *= 2;
@@ -1022,7 +1016,7 @@ cudaError_t launch_one(const CUtensorMap& k, const CUtensorMap& v, const Args& a
   constexpr auto kKernel = paged_attention_kernel<D, kWide, kStep, false>;
   cudaError_t e = allow_smem<kKernel>(smem_bytes(D, kWide));
   if (e != cudaSuccess) return e;
-  const long long most = sm_count() * blocks_per_sm(D, kWide) < kMostBlocks ? sm_count() * blocks_per_sm(D, kWide) : kMostBlocks;
+  const long long most = current_sm_count() * blocks_per_sm(D, kWide) < kMostBlocks ? current_sm_count() * blocks_per_sm(D, kWide) : kMostBlocks;
   const int blocks = static_cast<int>(pairs * a.pair_tiles < most ? pairs * a.pair_tiles : most);
   e = launch_kernel(kKernel, dim3(blocks), dim3(kThreads), smem_bytes(D, kWide), stream, k, v, a);
   if (e != cudaSuccess) return e;

@@ -16,9 +16,8 @@
 // k tokens) goes into a list; order, masses and the draw are then a matter of comparing its entries pair by pair.
 //
 // Where everything counts (no top-k, a large one, many equal values), the border of the top-k or of the nucleus is looked for by
-// histograms over equal steps of the value between the largest and the smallest one left: counts, or masses as three numbers of 15
-// bits, then the bin of the border alone, by pairs where it holds few values and in finer steps where it does not.
-#include <cfloat>
+// histograms over equal steps of the value between the largest and the smallest one left: counts, or masses as three numbers of up to 16
+// bits (sums of a block's 2^16 tokens stay within 32), then the bin of the border alone, by pairs where it holds few values and in finer steps where it does not.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "elem.cuh"
@@ -33,38 +32,45 @@ constexpr int kList = 512;                 // entries compared pair by pair
 constexpr int kFew = 256;                  // the largest k that takes the bound
 constexpr int kMany = 2048;                // tokens that a larger top-k leaves in a block, as a list
 constexpr int kMostBlocks = 8;             // of a row: the largest cluster that every device takes
-constexpr int kSliceBytes = 144 * 1024;    // of a row in a block: 2^18 numbers of 32 bits are eight blocks of 128 KB
+constexpr int kSliceBytes = 128 * 1024;    // of a row in a block: 2^16 tokens at most; 2^18 numbers of 32 bits are eight blocks
 using u64 = unsigned long long;
 constexpr u64 kOne = 1ull << 44;
 
-// Order of logits as unsigned numbers, NaN below -inf; bf16 in the upper half.
+// Order of logits as unsigned numbers, NaN below -inf, -0 as 0, +inf as the largest number; bf16 in the upper half.
 template <typename T>
 struct Key;
 template <>
 struct Key<float> {
   static constexpr uint32_t kMinusInf = 0x007fffffu;
   static __device__ __forceinline__ uint32_t of(uint32_t bits) {
-    const uint32_t u = __float_as_uint(__uint_as_float(bits) + 0.f);         // -0 is 0
+    const uint32_t u = __float_as_uint(__uint_as_float(bits) + 0.f);
     const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
-    return (bits & 0x7fffffffu) > 0x7f800000u ? 0u : k;
+    return (bits & 0x7fffffffu) > 0x7f800000u ? 0u : min(k, 0xff7fffffu);
   }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float(k ^ (~static_cast<uint32_t>(static_cast<int>(k) >> 31) | 0x80000000u));
   }
-  // keys of 16 bytes of logits, and back
-  static __device__ __forceinline__ uint4 pack(const uint32_t (&k)[4]) { return make_uint4(k[0], k[1], k[2], k[3]); }
+  // the key of a number or of one just below it
+  static __device__ __forceinline__ uint32_t near(float x) { return of(__float_as_uint(x)); }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ uint32_t largest(uint32_t m) { return m; }
   static __device__ __forceinline__ uint32_t unpack(const uint32_t (&w)[4], int e) { return w[e]; }
 };
 template <>
-struct Key<bf16> {
+struct Key<bf16> {                         // two at a time
   static constexpr uint32_t kMinusInf = 0x007f0000u;
-  static __device__ __forceinline__ uint32_t of(uint32_t bits) { return Key<float>::of(bits) & 0xffff0000u; }
+  static __device__ __forceinline__ uint32_t of(uint32_t bits) {
+    const __nv_bfloat162 x = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&bits), __nv_bfloat162(from_f32<bf16>(0.f), from_f32<bf16>(0.f)));
+    const uint32_t nan = __hneu2_mask(x, x), u = *reinterpret_cast<const uint32_t*>(&x);
+    const uint32_t k = u ^ ((u >> 15 & 0x00010001u) * 0xffffu | 0x80008000u);
+    return __vminu2(k & ~nan, 0xff7fff7fu);
+  }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float((k ^ (~static_cast<uint32_t>(static_cast<int>(k) >> 31) | 0x80000000u)) & 0xffff0000u);
   }
-  static __device__ __forceinline__ uint4 pack(const uint32_t (&k)[8]) {
-    return make_uint4(k[0] >> 16 | k[1], k[2] >> 16 | k[3], k[4] >> 16 | k[5], k[6] >> 16 | k[7]);
-  }
+  static __device__ __forceinline__ uint32_t near(float x) { return Key<float>::of(__float_as_uint(x)) & 0xffff0000u; }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  static __device__ __forceinline__ uint32_t largest(uint32_t m) { return max(m & 0xffff0000u, m << 16); }
   static __device__ __forceinline__ uint32_t unpack(const uint32_t (&w)[4], int e) { return e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16; }
 };
 // One order of all tokens: by value, ties by the lowest index.
@@ -152,10 +158,10 @@ struct Row {
   }
   // exp((x - max) / T) as a multiple of 2^-44, good to 2^-31 of itself: y = (x - max) 256 log2 e / T as a sum of two numbers, the
   // whole part n of its 256ths from the table, 2^(f / 256) = 1 + q of the rest by a polynomial, q in 2^-31ths. The largest has exactly
-  // 1; an infinite one counts as the largest number that there is. What lies below 2^-45, and -inf, shift everything out; nobody asks
-  // for the mass of NaN.
+  // 1. What lies below 2^-45, -inf and NaN shift everything out. Whole-number instructions run at half the rate of the others here: what
+  // can be had from products and sums is.
   __device__ __forceinline__ u64 mass(uint32_t key) const {
-    const float x = fminf(Key<T>::value(key), FLT_MAX), d = x - top;
+    const float x = Key<T>::value(key), d = x - top;
     float rest = 0.f;
     if constexpr (sizeof(T) == 4) {                       // what the difference has lost (of bf16 numbers: nothing that counts)
       const float back = d - x;
@@ -308,7 +314,21 @@ __device__ __forceinline__ int nth_equal(const Row<T, kThreads>& r, uint32_t key
   return found == ~0ull ? 0x7fffffff : static_cast<int>(found);
 }
 
-// The last token, in descending order through the keys from `high` down to `low` (both there), that has at most so much ahead of it:
+// The last number from a to b for which `holds`, which does so up to some number and not behind it; a where it never does. A warp.
+template <typename F>
+__device__ __forceinline__ uint32_t last_with(uint32_t a, uint32_t b, F holds, int lane) {
+  while (a < b) {
+    const uint32_t step = (b - a) / 32 + 1, at = a + min(lane * step, b - a);
+    const unsigned yes = __ballot_sync(0xffffffffu, holds(at));
+    const uint32_t first = a + (yes ? min((31 - __clz(yes)) * step, b - a) : 0);
+    b = first + min(step - 1, b - first);
+    if (!yes) b = a;
+    a = first;
+  }
+  return a;
+}
+
+// The last token, in descending order through the keys from `high` down to `low`, that has at most so much ahead of it:
 // `left` tokens, or (kMass) that fraction of the mass of all. For counts only the key of the result means something.
 template <bool kMass, typename T, int kThreads>
 __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, uint32_t high, u64 left) {
@@ -320,7 +340,7 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
     // equal steps of the value behind the largest, which has bin 0 to itself: every turn leaves it behind or ends with it
     const float most = Key<T>::value(high);
     const float steps = static_cast<float>((kBins - 2) / (static_cast<double>(most) - static_cast<double>(Key<T>::value(low))));
-    // 2^23 + 1 and up: rounded to whole numbers, in the low bits (fminf takes the number where the other is NaN)
+    // 2^23 + 1 and up: rounded to whole numbers, in the low bits (0 times an infinite number of steps: fminf takes the other)
     auto bin_of = [&](uint32_t k) {
       const float at = fminf((most - Key<T>::value(k)) * steps, kBins - 2.f) + 8388609.f;
       return k == high ? 0 : __float_as_int(at) & (kBins - 1);
@@ -333,9 +353,9 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
       const u64 m = kMass ? r.mass(k) : 1;
       if (k - low > high - low) return;
       if constexpr (kMass) {
-        atomicAdd(&s.hist[0][b], static_cast<unsigned>(m & 0x7fff));
-        atomicAdd(&s.hist[1][b], static_cast<unsigned>(m >> 15 & 0x7fff));
-        atomicAdd(&s.hist[2][b], static_cast<unsigned>(m >> 30));
+        atomicAdd(&s.hist[0][b], static_cast<unsigned>(m & 0xffff));
+        atomicAdd(&s.hist[1][b], static_cast<unsigned>(m) >> 16);
+        atomicAdd(&s.hist[2][b], static_cast<unsigned>(m >> 32));
       } else {
         atomicAdd(&s.hist[0][b], 1u);
       }
@@ -348,8 +368,8 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
 #pragma unroll
         for (int e = 0; e < (kMass ? 3 : 1); ++e) {
           const u64 two = peer64(&s.hist[e][2 * tid], b);
-          held[0] += (two & 0xffffffffu) << 15 * e;
-          held[1] += two >> 32 << 15 * e;
+          held[0] += (two & 0xffffffffu) << 16 * e;
+          held[1] += two >> 32 << 16 * e;
         }
       }
     }
@@ -366,16 +386,8 @@ __device__ __forceinline__ u64 border(const Row<T, kThreads>& r, uint32_t low, u
     // the bin as a range of keys: bins fall as keys rise, so its ends are the last keys above it and up to it
     if (tid < 64) {
       const int least = bin + (tid < 32);                 // warp 0: the last key of a larger bin; warp 1: of this or a larger one
-      uint32_t a = low, b = high;
-      const bool any = bin_of(low) >= least;
-      while (any && a < b) {
-        const uint32_t step = (b - a) / 32 + 1, k = a + min((tid & 31) * step, b - a);
-        const unsigned yes = __ballot_sync(0xffffffffu, bin_of(k) >= least);
-        const uint32_t first = a + min((31 - __clz(yes)) * step, b - a);
-        b = first + min(step - 1, b - first);
-        a = first;
-      }
-      if ((tid & 31) == 0) s.ends[tid >> 5] = tid < 32 ? (any ? a + 1 : low) : a;
+      const uint32_t key = last_with(low, high, [&](uint32_t k) { return bin_of(k) >= least; }, tid & 31);
+      if ((tid & 31) == 0) s.ends[tid >> 5] = tid >= 32 ? key : bin_of(low) >= least ? key + 1 : low;
     }
     __syncthreads();
     const uint32_t bottom = s.ends[0], span = s.ends[1] - bottom;
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   uint4* s_data = s_dyn + (sizeof(s) + 15) / 16;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < 256) s.powers[tid] = static_cast<unsigned>(exp2(tid / 256.0 + 31.0) + 0.5);
-  if (tid == 0) s.key = 0, s.low = 0xffffffffu, s.tau = 0, s.count = 0;
+  if (tid == 0) s.key = 0, s.tau = 0, s.count = 0, s.low = 0xffffffffu;
   __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
@@ -501,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   const int top_k = p.top_ks ? p.top_ks[b] : p.top_k;
 
   // the row's share into shared memory, NaN behind its end
-  uint32_t high = 0, low = 0xffffffffu;
+  uint32_t high = 0;
   const bool whole = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   constexpr int kAhead = 4;                               // loads of a thread under way
   for (int v0 = warp * stretch + lane * kVec; v0 < (warp + 1) * stretch; v0 += kAhead * 32 * kVec) {
@@ -524,17 +536,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
     for (int a = 0; a < kAhead; ++a) {
       const int v = v0 + a * 32 * kVec;
       if (v >= (warp + 1) * stretch) continue;
-      const uint32_t w[4] = {q[a].x, q[a].y, q[a].z, q[a].w};
-      uint32_t keys[kVec];
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        keys[e] = Key<T>::of(sizeof(T) == 4 ? w[e & 3] : e & 1 ? w[e / 2 % 4] & 0xffff0000u : w[e / 2 % 4] << 16);
-        high = max(high, keys[e]);
-        low = min(low, keys[e] > Key<T>::kMinusInf ? keys[e] : 0xffffffffu);
-      }
-      s_data[v / kVec] = Key<T>::pack(keys);
+      const uint4 k = make_uint4(Key<T>::of(q[a].x), Key<T>::of(q[a].y), Key<T>::of(q[a].z), Key<T>::of(q[a].w));
+      high = Key<T>::most(high, Key<T>::most(Key<T>::most(k.x, k.y), Key<T>::most(k.z, k.w)));
+      s_data[v / kVec] = k;
     }
   }
+  high = Key<T>::largest(high);
   // the largest lane maxima of every warp
   const int warps = min(r.blocks * kWarps, (V + stretch - 1) / stretch);     // that have tokens
   const int draws = (2 * top_k + warps - 1) / warps;
@@ -549,17 +556,10 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
     }
   }
   high = __reduce_max_sync(0xffffffffu, high);
-  low = __reduce_min_sync(0xffffffffu, low);
-  if (lane == 0) {
-    atomicMax(&s.key, high);
-    atomicMin(&s.low, low);
-  }
+  if (lane == 0) atomicMax(&s.key, high);
   r.sync();
-  uint32_t best = 0, least = 0xffffffffu;
-  for (int c = 0; c < r.blocks; ++c) {
-    best = max(best, r.blocks > 1 ? peer32(&s.key, c) : s.key);
-    least = min(least, r.blocks > 1 ? peer32(&s.low, c) : s.low);
-  }
+  uint32_t best = 0;
+  for (int c = 0; c < r.blocks; ++c) best = max(best, r.blocks > 1 ? peer32(&s.key, c) : s.key);
   if (few) {                                              // the k-th largest of them
     const int each = min(kWarps, warps) * draws, n = warps * draws;
     if (tid < n) s.all_tops[tid] = r.blocks > 1 ? peer32(&s.tops[tid % each], tid / each) : s.tops[tid];
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   r.sync();
   const uint32_t reach = max(s.tau, Key<T>::kMinusInf + 1);
   r.best = best;
-  r.top = fminf(Key<T>::value(best), FLT_MAX);
+  r.top = Key<T>::value(best);
   const double rate = fmin(369.32993046757462 / static_cast<double>(temperature), 1e38);   // 256 log2 e, and finite: 0 times it is 0
   r.rate = static_cast<float>(rate);
   r.rate_low = static_cast<float>(rate - static_cast<double>(r.rate));
@@ -658,16 +658,32 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
     return;
   }
   if (top_k > 0 && top_k < V) {
-    from = max(from, static_cast<uint32_t>(border<false>(r, least, best, static_cast<u64>(top_k - 1)) >> 32));
+    uint32_t least = 0xffffffffu;                         // the smallest value that there is
+    r.each([&](uint32_t k, int) { least = min(least, k > Key<T>::kMinusInf ? k : 0xffffffffu); });
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) atomicMin(&s.low, least);
+    r.sync();
+    for (int c = 0; c < r.blocks; ++c) least = min(least, r.blocks > 1 ? peer32(&s.low, c) : s.low);
+    r.sync();
+    from = static_cast<uint32_t>(border<false>(r, least, best, static_cast<u64>(top_k - 1)) >> 32);
     list_from(r, from);
   }
   u64 last = token(from, 0x7fffffff);                     // the last token that stays
-  if (top_p < 1.f) last = border<true>(r, max(from, least), best, share);
+  // 45 octaves below the largest there are no masses left
+  if (top_p < 1.f) last = border<true>(r, max(from, Key<T>::near(r.top - 32.f * temperature)), best, share);
+  if (least_mass > 0) {                                   // min-p as a token: weights rise with the keys
+    if (warp == 0) {
+      const uint32_t key = last_with(from, best, [&](uint32_t k) { return r.mass(k) < least_mass; }, lane);
+      if (lane == 0) s.key = r.mass(from) < least_mass ? key + 1 : from;
+    }
+    __syncthreads();
+    last = max(last, token(s.key, 0x7fffffff));
+  }
   const uint32_t last_key = last >> 32;
   const int last_equal = static_cast<int>(~static_cast<uint32_t>(last));
-  auto held = [&](uint32_t k, int i) -> u64 {
+  auto held = [&](uint32_t k, int i) -> u64 {             // no branch: hardly ever would a whole warp skip one
     const u64 w = r.mass(k);
-    return k < last_key || (k == last_key && i > last_equal) || w < least_mass ? 0 : w;
+    return k > last_key || (k == last_key && i <= last_equal) ? w : 0;
   };
   u64 own = 0;
   r.each([&](uint32_t k, int i) { own += held(k, i); });
@@ -692,12 +708,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
       before += __shfl_sync(0xffffffffu, upto, 31);
     });
   }
-}
-
-int sm_count() {
-  int device = 0, n = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 148;
-  return n;
 }
 
 template <typename T, int kThreads>
@@ -735,7 +745,7 @@ template <typename T>
 cudaError_t launch_one(const void* logits, long long ld, int B, int V, const cd_sample& p, int64_t* ids, float* probs, cudaStream_t stream) {
   int blocks = 1;
   while (static_cast<long long>(V) * sizeof(T) > static_cast<long long>(blocks) * kSliceBytes) blocks *= 2;
-  while (blocks < kMostBlocks && 2LL * blocks * B <= sm_count() && V / (2 * blocks) >= 4096) blocks *= 2;
+  while (blocks < kMostBlocks && 2LL * blocks * B <= current_sm_count() && V / (2 * blocks) >= 4096) blocks *= 2;
   const T* x = static_cast<const T*>(logits);
   long long* to = reinterpret_cast<long long*>(ids);
   return V / blocks > 16384 ? launch_blocks<T, 1024>(blocks, x, ld, B, V, p, to, probs, stream)

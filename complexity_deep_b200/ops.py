@@ -1584,14 +1584,18 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     B, V = logits.shape
     if V > 1 << 18:
         raise RuntimeError("sample_tokens: at most 262144 logits a row")
-    each = [None, None, None, None]                       # tensors' addresses; the numbers of the others
-    one = [1.0, 1.0, 0.0, 0]
-    for i, rule in enumerate((temperature, top_p, min_p, top_k)):
-        if isinstance(rule, torch.Tensor):
-            each[i] = _on(rule, ("temperature", "top_p", "min_p", "top_k")[i], torch.float32 if i < 3 else torch.int32, device, (B,))
-        else:
-            one[i] = rule
-    r = _lib.Sample(_on(uniform, "uniform", torch.float32, device, (B,)), *each, *one)
+    f32, tensor = torch.float32, torch.Tensor
+    # a tensor's address, or the number of all rows
+    temperatures = top_ks = top_ps = min_ps = None
+    if isinstance(temperature, tensor):
+        temperatures, temperature = _on(temperature, "temperature", f32, device, (B,)), 1.0
+    if isinstance(top_k, tensor):
+        top_ks, top_k = _on(top_k, "top_k", torch.int32, device, (B,)), 0
+    if isinstance(top_p, tensor):
+        top_ps, top_p = _on(top_p, "top_p", f32, device, (B,)), 1.0
+    if isinstance(min_p, tensor):
+        min_ps, min_p = _on(min_p, "min_p", f32, device, (B,)), 0.0
+    r = _lib.Sample(_on(uniform, "uniform", f32, device, (B,)), temperatures, top_ps, min_ps, top_ks, temperature, top_p, min_p, top_k)
     ids, probs = uniform.new_empty(B, dtype=torch.int64), uniform.new_empty(B)
     if B:
         with _Span("sample_tokens"):

@@ -116,6 +116,17 @@ def test_infinities_and_nan():
     assert ids.tolist() == [0, 0] and probs.tolist() == [0.0, 0.0]
 
 
+def test_small_values_and_zeros():
+    """Zeros of both signs are equal; subnormal numbers and their neighbours are not."""
+    g = torch.Generator().manual_seed(6)
+    for dtype in (torch.bfloat16, torch.float32):
+        pool = torch.tensor([0.0, -0.0, 1e-39, -1e-39, 2e-39, 1e-38, -3e-38, 1e-20]).to(dtype)
+        x = pool[torch.randint(0, 8, (4, 1500), generator=g)]
+        u = torch.rand(4, generator=g)
+        for rules in ((1.0, 100, 1.0, 0.0), (1e-38, 0, 0.6, 0.0), (1e-20, 700, 0.5, 0.0), (2e-39, 0, 1.0, 0.2), (0.0, 0, 1.0, 0.0)):
+            _check(x, u, *rules)
+
+
 def test_odd_rules_and_strides():
     """Rules at the ends of their ranges and beyond, given numbers outside [0, 1), one row of logits for many draws."""
     from complexity_deep_b200 import ops
