@@ -71,6 +71,16 @@ def test_rows_beyond_what_a_block_holds():
     _run([60000, 700], 1, 64, 256, 650, 100, seed=7, width=256)
     _run([3000, 60000, 64], 2, 8, 64, 2000, 0, seed=8, width=1024, in_place=False)
     _run([60000], 1, 64, 64, 30000, 5, seed=9, width=1000, ties=True, order="rows")
+    _run([700, 60000, 50, 3], 40, 8, 64, 600, 3, seed=10, width=1024, ties=True)          # one block a pair
+
+
+@pytest.mark.parametrize("rows,keep", [(520, 256), (2100, 1050), (4200, 300), (9000, 4500), (17000, 16000), (33000, 1)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_several_blocks_a_pair(rows, keep, ties):
+    """Clusters of 2 to 8 blocks: shares of rows that end anywhere, equal weights across their borders, sequences shorter than the
+    table (blocks without rows), both ways of writing the outputs."""
+    _run([rows, rows // 2, 3, keep + 1], 1, 8, 16, keep, 1, seed=rows, ties=ties, in_place=ties)
+    _run([rows - 7], 3, 16, 32, keep, keep // 3, seed=keep, ties=ties, in_place=not ties, width=-(-rows // 32) + 9)
 
 
 def test_odd_weights():
