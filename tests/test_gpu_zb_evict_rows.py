@@ -67,7 +67,7 @@ def test_layers_and_long():
 
 
 def test_rows_beyond_what_a_block_holds():
-    """Tables of more than 53 248 rows: keys are read again, lists lie in the workspace; also with several blocks a pair."""
+    """Shares of more than 49 152 rows: keys are read again, lists lie in the workspace; also with several blocks a pair."""
     _run([60000, 700], 1, 64, 256, 650, 100, seed=7, width=256)
     _run([3000, 60000, 64], 2, 8, 64, 2000, 0, seed=8, width=1024, in_place=False)
     _run([60000], 1, 64, 64, 30000, 5, seed=9, width=1000, ties=True, order="rows")
@@ -81,6 +81,26 @@ def test_several_blocks_a_pair(rows, keep, ties):
     table (blocks without rows), both ways of writing the outputs."""
     _run([rows, rows // 2, 3, keep + 1], 1, 8, 16, keep, 1, seed=rows, ties=ties, in_place=ties)
     _run([rows - 7], 3, 16, 32, keep, keep // 3, seed=keep, ties=ties, in_place=not ties, width=-(-rows // 32) + 9)
+
+
+@pytest.mark.parametrize("pairs,rows", [(149, 400), (149, 3990), (149, 4100), (600, 200), (600, 2600), (600, 60)])
+def test_many_pairs(pairs, rows):
+    """More pairs than SMs, and than four an SM: blocks of 128, 256 and 1 024 threads."""
+    from complexity_deep_b200 import ops
+    g = torch.Generator().manual_seed(rows)
+    width = -(-rows // 16)
+    pool = torch.randn(pairs * width, 1, 16, 8, generator=g).to(torch.bfloat16).cuda()
+    table = torch.arange(pairs * width, dtype=torch.int32, device="cuda").view(pairs, width)
+    w, pos = torch.randn(pairs, 1, width * 16, generator=g).exp(), torch.rand(pairs, 1, width * 16, generator=g).argsort(-1).to(torch.int32)
+    keep, n = rows // 2, torch.full((pairs,), rows, dtype=torch.int32, device="cuda")
+    wd, pd, kd, vd = w.cuda(), pos.cuda(), pool.clone(), pool.clone() + 1
+    ops.evict_rows_(kd, vd, table, n, n, wd, pd, keep, 7)
+    flat, moved = pool.view(pairs, width * 16, 8).cpu(), kd.view(pairs, width * 16, 8).cpu()
+    for b in list(range(0, pairs, 37)) + [pairs - 1]:
+        src = torch.tensor(cases.evict(w[b, 0].tolist(), pos[b, 0].tolist(), rows, rows - 7, keep))
+        assert torch.equal(moved[b, :keep], flat[b, src]) and torch.equal(moved[b, keep:], flat[b, keep:])
+        assert torch.equal(wd[b, 0, :keep].cpu(), w[b, 0, src]) and torch.equal(pd[b, 0, :keep].cpu(), pos[b, 0, src])
+    assert torch.equal(vd.view(pairs, width * 16, 8).cpu()[:, :keep], (moved + 1)[:, :keep])
 
 
 def test_odd_weights():
