@@ -94,6 +94,10 @@ def paged_generate(model, prompts: Sequence[torch.Tensor], max_new_tokens: int =
     """Continues prompts of any lengths side by side; each stops at the end token (the config's, unless given) or after
     `max_new_tokens`.  temperature 0: greedy.  keep: sequences are cut back to that many rows whenever one has an eighth
     (at least a page) more.  Returns prompt and continuation of each."""
+    if not prompts or min(len(p) for p in prompts) < 1:
+        raise ValueError("paged_generate needs prompts of at least one token")
+    if max_new_tokens < 1:
+        return [list(map(int, p)) for p in prompts]
     eos = getattr(model.config, "eos_token_id", None) if eos_token_id is None else eos_token_id
     device = next(model.parameters()).device
     longest = max(len(p) for p in prompts)

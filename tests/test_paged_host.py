@@ -178,3 +178,11 @@ def test_command_line_prompts():
     for texts, equal in ((["1,2", "3"], True), (["1", ""], False)):
         with pytest.raises(SystemExit):
             cli.parse_prompts(texts, equal)
+
+
+def test_generate_without_work():
+    from complexity_deep_b200.models import paged_generate
+    assert paged_generate(None, [[3, 1], torch.tensor([4])], max_new_tokens=0) == [[3, 1], [4]]
+    for prompts in ([], [[3], []]):
+        with pytest.raises(ValueError, match="at least one token"):
+            paged_generate(None, prompts)
