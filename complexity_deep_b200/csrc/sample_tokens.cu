@@ -20,7 +20,8 @@
 // the upper ones with what the lower carry. Then the bin of the border alone: in finer steps where it holds many values; otherwise as a
 // list, of which every warp weighs what lies ahead of one, 32 at a time (294 values: 7 000 clocks; all pairs of them 10 700).
 // The draw weighs what has stayed once more: picked from 32 tokens of a lane at a time, 18 000 clocks for 100 000 tokens of which a
-// third stays, 24 000 with a weight for every token.
+// third stays, 24 000 with a weight for every token. The warp's stretch in which it ends is taken by the whole block: 2 200 clocks, 8 000
+// for the warp alone.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "elem.cuh"
@@ -151,6 +152,15 @@ struct Row {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int e = 0; e < kVec; ++e) f(Key<T>::unpack(w, e), begin + v + e);
+  }
+  // f(key, token index) for the one token at place v
+  template <typename F>
+  __device__ __forceinline__ void one(int v, F f) const {
+    if (many >= 0) {
+      at(v, f);
+    } else {
+      f(Key<T>::at(data, v), begin + v);
+    }
   }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
@@ -755,26 +765,28 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_tokens_kerne
   u64 own = 0;
   r.each_that([&](uint32_t k) { return k >= last_key; }, [&](uint32_t k, int i) { own += held(k, i); });
   const u64 total = row_sum(r, own), target = __umul64hi(u, total);
-  const u64 mine = s.sums[warp];
-  u64 before = s.before + warp_sum(lane < warp ? s.sums[lane] : 0);
-  if (before <= target && target < before + mine) {       // in this warp's stretch
-    r.steps([&](int v) {
-      u64 w = 0;
-      if (v < r.to()) r.at(v, [&](uint32_t k, int i) { w += held(k, i); });
-      const u64 upto = warp_upto(w);
-      u64 at = before + upto - w;
-      if (w > 0 && at <= target && target < at + w)
-        r.at(v, [&](uint32_t k, int i) {
-          const u64 e = held(k, i);
-          if (e > 0 && at <= target && target < at + e) {
-            ids[b] = i;
-            probs[b] = static_cast<float>(static_cast<double>(e) / static_cast<double>(total));
-          }
-          at += e;
-        });
-      before += __shfl_sync(0xffffffffu, upto, 31);
+  // the warp's stretch that it falls into, of which every thread of the block then takes a few neighbouring tokens
+  const u64 of_warp = lane < kWarps ? s.sums[lane] : 0, upto = s.before + warp_upto(of_warp);
+  const unsigned beyond = __ballot_sync(0xffffffffu, upto > target);
+  if (s.before > target || beyond == 0) return;           // in another block
+  const int pick = __ffs(beyond) - 1;
+  const u64 ahead = __shfl_sync(0xffffffffu, upto - of_warp, pick);
+  const int first = pick * r.stretch, places = (r.many < 0 ? first + r.stretch : min(r.many, first + r.stretch)) - first;
+  const int each = (places + kThreads - 1) / kThreads;
+  const int v0 = first + min(places, tid * each), v1 = first + min(places, (tid + 1) * each);
+  u64 some = 0;
+  for (int v = v0; v < v1; ++v) r.one(v, [&](uint32_t k, int i) { some += held(k, i); });
+  u64 at = ahead + block_before(some, s.sums);
+  if (at > target || target >= at + some) return;
+  for (int v = v0; v < v1; ++v)
+    r.one(v, [&](uint32_t k, int i) {
+      const u64 e = held(k, i);
+      if (at <= target && target < at + e) {
+        ids[b] = i;
+        probs[b] = static_cast<float>(static_cast<double>(e) / static_cast<double>(total));
+      }
+      at += e;
     });
-  }
 }
 
 template <typename T, int kThreads>
@@ -804,10 +816,10 @@ cudaError_t launch_blocks(int blocks, const T* logits, long long ld, int B, int 
   return cudaLaunchKernelEx(&cfg, kKernel, logits, ld, V, blocks, slice, stretch, p, ids, probs);
 }
 
-// As many blocks a row as its size asks for, and more while there is an SM for each and 4 096 tokens. us, 1 / 2 / 4 / 8 blocks of 512
-// threads: 1 x 32 000 11.7 / 10.8 / 9.7 / 9.8, 32 x 100 000 22.6 / 17.0 / 14.8 / 19.3 (two an SM), nucleus of 64 x 100 000
-// - / 68 / 91 / 135. Long shares take 1 024 threads: the nucleus 61, 256 x 32 000 in 32 bits 57 (62); short ones do not (1 x 32 000,
-// 4 blocks: 11.6).
+// As many blocks a row as its size asks for, and more while there is an SM for each and 4 096 tokens; long shares take 1 024 threads.
+// us, 1 / 2 / 4 / 8 blocks: of 512 threads 1 x 32 000 9.3 / 9.4 / 9.0 / 9.5, 32 x 100 000 - / 13.3 / 14.4 / 16.5, nucleus of 64 x 100 000
+// - / 73 / 76 / 115, 256 x 32 000 in 32 bits with rules by row 51 / 48 / 67 / 124; of 1 024 threads 10.1 / 10.6 / 10.4 / 11.0,
+// - / 14.3 / 12.4 / 32.7, - / 51 / 74 / 160, 46 / 68 / 111 / 259.
 template <typename T>
 cudaError_t launch_one(const void* logits, long long ld, int B, int V, const cd_sample& p, int64_t* ids, float* probs, cudaStream_t stream) {
   int blocks = 1;
