@@ -825,9 +825,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 constexpr int kMostBlocks = 2 * 160;
 constexpr int kFinishThreads = 256;
 
-// What a stretch has left: the pairs at its two ends where they are cut (their output, by the block behind the first cut), half of
-// the warps each; then the weights of its tiles, a warp a tile. A chain of three loads, each for all that the one before has made
-// known: 3 us, where asking for things as they came took 9 (32 sequences, 3 600 tiles).
+// What a stretch has left: the maxima and sums of the pairs at its two ends where they are cut, half of the warps each; its share of the
+// columns of the pair at its beginning (those behind a pair's first cut have a share each, neighbouring lanes some parts of a
+// column each); then the weights of its tiles, a warp a tile. A chain of three loads, each for all that the one before has made known:
+// 3 us, where asking for things as they came took 9 (32 sequences, 3 600 tiles). One block for all columns of a pair took long where few pairs
+// are cut into many parts: 1 x 14 204 rows, 16 heads of 128, 124 us a call (24 now), 2 x 32 768, 8 x 2 x 128, 50.6 (48.6).
 template <bool kStep>
 __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args a, int D) {
   constexpr int kHalf = kFinishThreads / 2, kAhead = 4;
@@ -849,21 +851,34 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args
 #pragma unroll
     for (int g = 0; g < kAhead; ++g) ahead[g] = *reinterpret_cast<const float2*>(scores + min(g, G - 1) * kTile);
   }
-  const int half = tid >= kHalf, in_half = tid - half * kHalf;
+  const bool same = st.end[0].pair == st.end[1].pair;     // all warps for the one
+  const int half = !same && tid >= kHalf;
   const End p = half ? st.end[1] : st.end[0];
-  const bool cut = p.first < p.last && !(half && st.end[0].pair == p.pair);
+  const bool cut = p.first < p.last;
   const int parts = p.last - p.first + 1, size = part_floats(G, D);
   auto part = [&](int x) { return a.part + (2LL * (p.first + x) + (x == 0 ? p.second : 0)) * size; };
-  const bool writes = cut && c == p.first + 1;
-  // four columns a thread, of the first parts
+  // columns: four a lane, `each` lanes of them; a lane's first parts are asked for here
+  const End b = st.end[0];
+  const int b_parts = b.last - b.first + 1;
+  auto b_part = [&](int x) { return a.part + (2LL * (b.first + x) + (x == 0 ? b.second : 0)) * size; };
+  int from = 0, to = 0, shift = 0;
+  if (b.first < c) {
+    const unsigned all = G * D / 4, share = (all + b_parts - 2) / static_cast<unsigned>(b_parts - 1);
+    from = min(all, (c - b.first - 1) * share);
+    to = min(all, from + share);
+    while (shift < 5 && 1 << shift < b_parts && (to - from) << (shift + 1) <= kFinishThreads) ++shift;
+  }
+  const int each = 1 << shift, turn = tid & (each - 1);
+  int i = from + (tid >> shift);
   float4 column[kAhead];
-  if (writes && 4 * in_half < G * D) {
+  if (i < to) {
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) column[x] = *reinterpret_cast<const float4*>(part(min(x, parts - 1)) + 4 * in_half);
+    for (int x = 0; x < kAhead; ++x) column[x] = *reinterpret_cast<const float4*>(b_part(min(turn + x * each, b_parts - 1)) + 4 * i);
   }
   if (cut) {
-    for (int g = in_half >> 5; g < G; g += kHalf / 32) {
+    for (int g = (tid - half * kHalf) >> 5; g < G; g += (same ? kFinishThreads : kHalf) / 32) {
       float top = -FLT_MAX, sum = 0.f;
+#pragma unroll 4
       for (int x = lane; x < parts; x += 32) {
         const float2 ml = *reinterpret_cast<const float2*>(part(x) + G * D + 2 * g);
         const float next = fmaxf(top, ml.x);
@@ -882,25 +897,35 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args
     }
   }
   __syncthreads();
-  if (writes) {
-    for (int i = 4 * in_half; i < G * D; i += 4 * kHalf) {
-      const int g = i / D;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto add = [&](const float4& p4, float f) {
-        v.x += p4.x * f;
-        v.y += p4.y * f;
-        v.z += p4.z * f;
-        v.w += p4.w * f;
-      };
+  for (int i0 = from; i0 < to; i0 += kFinishThreads >> shift, i += kFinishThreads >> shift) {     // the same for all lanes
+    const bool has = i < to;
+    const int g = has ? i >> (D == 64 ? 4 : 5) : 0;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& p4, float f) {
+      v.x += p4.x * f;
+      v.y += p4.y * f;
+      v.z += p4.z * f;
+      v.w += p4.w * f;
+    };
+    if (has) {
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
-        if (i > 4 * in_half) column[x] = *reinterpret_cast<const float4*>(part(min(x, parts - 1)) + i);
-        if (x < parts) add(column[x], s_scale[half][x * G + g]);
+        const int at = turn + x * each;
+        if (i0 > from) column[x] = *reinterpret_cast<const float4*>(b_part(min(at, b_parts - 1)) + 4 * i);
+        if (at < b_parts) add(column[x], s_scale[0][at * G + g]);
       }
 #pragma unroll 4
-      for (int x = kAhead; x < parts; ++x) add(*reinterpret_cast<const float4*>(part(x) + i), s_scale[half][x * G + g]);
-      const float inv = s_final[half][g].y;
-      *reinterpret_cast<uint2*>(a.out + static_cast<long long>(p.pair) * G * D + i) =
+      for (int at = turn + (kAhead << shift); at < b_parts; at += each) add(*reinterpret_cast<const float4*>(b_part(at) + 4 * i), s_scale[0][at * G + g]);
+    }
+    for (int o = 1; o < each; o <<= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+      v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
+    }
+    if (has && turn == 0) {
+      const float inv = s_final[0][g].y;
+      *reinterpret_cast<uint2*>(a.out + static_cast<long long>(b.pair) * G * D + 4 * i) =
           make_uint2(bf_pack(v.x * inv, v.y * inv), bf_pack(v.z * inv, v.w * inv));
     }
   }

@@ -70,6 +70,13 @@ def test_line_of_tiles(G, D, weights):
     _attend([0] + [(97 * i) % 260 for i in range(130)] + [0], 3, G, D, 16, seed=G + 1, weights=weights, order="rows")
 
 
+@pytest.mark.parametrize("G,D", [(1, 64), (2, 128), (5, 64), (16, 128)])
+@pytest.mark.parametrize("lengths", [[19000], [15000, 9000, 40], [2600] * 17])
+def test_pairs_cut_between_most_blocks(lengths, G, D):
+    """One head of keys: a part of a pair from hundreds of blocks, from about a hundred, from some twenty."""
+    _attend(lengths, 1, G, D, 64, seed=G, weights=G % 2 == 1)
+
+
 def test_strides_and_shared_pages():
     """Pools that are every other page and a part of the heads of larger ones, a table that is a part of a wider one, two
     sequences that share their first pages."""
