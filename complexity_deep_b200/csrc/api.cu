@@ -1037,7 +1037,7 @@ static int paged_attention(const cd_paged* c, const cd_paged_step* step, const v
   if (reinterpret_cast<uintptr_t>(c->weights) & 7) return CD_ERR_INVALID;
   const size_t need = paged_attention_workspace_bytes(B, hq, hkv, D, c->page, c->width, c->weights != nullptr);
   if (need && (!ws || !aligned16(ws) || ws_bytes < need)) return CD_ERR_INVALID;
-  if ((static_cast<long long>(c->width) * c->page + 63) / 64 * B * hkv > 0x7fffffffLL) return CD_ERR_UNSUPPORTED;   // tiles are counted in 32 bits
+  if (((static_cast<long long>(c->width) * c->page + 63) / 64 + 4) * B * hkv > 0x7fffffffLL) return CD_ERR_UNSUPPORTED;   // tiles, and what a pair adds to them, are counted in 32 bits
   int* status = device_status_word();
   if (!status) return CD_ERR_CUDA;
   const cudaError_t e = launch_paged_attention(*c, step, q, q_stride, scale, B, hq, hkv, D, out, ws, status, as_stream(stream));

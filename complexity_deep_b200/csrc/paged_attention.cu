@@ -9,7 +9,7 @@
 // significant bits) at no cost. More heads take two products instead.
 //
 // Work is cut into tiles of 64 rows; all tiles of all (sequence, KV head) pairs stand in one line, of which every block takes an equal
-// stretch, whatever the lengths are. A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
+// stretch, whatever the lengths are (a pair's beginning counts as a few tiles: pair_units). A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
 // block, which a second kernel adds in order (results do not depend on timing). A warp feeds tiles to the ring with TMA (a
 // box per page, 128-byte swizzle), four warps take 16 rows of a tile each, with a running maximum and sum of their own.
 //
@@ -59,6 +59,12 @@ __host__ __device__ constexpr int smem_bytes(int D, bool wide) {
   return 1024 + stages_of(D, wide) * stage_bytes(D) + merge_bytes(D, wide) + query_bytes(D, wide);
 }
 
+// What beginning a pair costs, in tiles: of the line, these come ahead of the pair's own. Without them a stretch of many short pairs holds
+// all others up. us a step with 0 / 1 / 2 / 4: 64 sequences of 32 to 2 047 rows, 8 x 2 x 128, 56 / 43 / 37 / 37, 16 of them empty 40 / 30 /
+// 26 / 27, 32 of 256 to 2 047 with weights 31.9 / 30.8 / 30.8 / 31.5, 64 x 1 000 to 16 384 264 / 267 / 266 / 270; of 16 heads, 0 / 1 / 3 / 4 / 5:
+// 55 of 1 197 and eight empty ones, 4 x 16 x 128, 133 / 84 / 62 / 62 / 63, 64 of 250 to 4 000 66 / 61 / 60 / 61 / 62.
+__host__ __device__ constexpr int pair_units(bool wide) { return wide ? 3 : 2; }
+
 // For the second kernel: a block's stretch and the pairs at its ends, all that it has to know before it can ask for anything.
 struct End {
   int pair;
@@ -66,7 +72,7 @@ struct End {
   int second;             // whether the first of them had begun with another pair
 };
 struct __align__(16) Stretch {
-  int blocks, begins, ends, pad;          // blocks that have one; this block's tiles
+  int blocks, begins, ends, pad;          // of the line; this block's tiles
   End end[2];
 };
 
@@ -93,7 +99,7 @@ struct Args {
 // Floats of a part: the heads' columns, then their maxima and sums.
 __host__ __device__ constexpr int part_floats(int G, int D) { return (G * (D + 2) + 3) / 4 * 4; }
 
-// Equal stretches of a line of `units` tiles: the first ones are a tile longer where it does not divide.
+// Equal stretches of a line of `units`: the first ones are one longer where it does not divide.
 struct Line {
   unsigned each, longer;
   __device__ __forceinline__ Line(unsigned units, unsigned blocks) : each(units / blocks), longer(units % blocks) {}
@@ -119,11 +125,11 @@ __device__ __forceinline__ int tiles_of(int rows) { return rows > 0 ? (rows + kT
 // A block's way along its stretch.
 struct Walk {
   int b, h, t, rows;
-  int left;               // tiles of the stretch from here on
+  int left;               // units of the stretch from here on
 };
-template <bool kStep>
+template <bool kWide, bool kStep>
 __device__ __forceinline__ void next_pair(const Args& a, Walk& w, int taken) {
-  w.left -= taken;
+  w.left -= taken + pair_units(kWide);
   w.t = 0;
   if (++w.h < a.hkv) return;
   w.h = 0;
@@ -304,10 +310,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(D, kWide))
 paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
   constexpr int kStages = stages_of(D, kWide), kHalf = kTile * D * 2;
   constexpr int kHeads = kWide ? 2 : 1;                   // of a lane
-  constexpr int kFloats = lane_floats(D, kWide);
+  constexpr int kFloats = lane_floats(D, kWide), kPair = pair_units(kWide);
   extern __shared__ unsigned char s_dyn[];
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_query, s_query_taken;
-  __shared__ int s_scan[kThreads / 32];
+  __shared__ int2 s_scan[kThreads / 32];
+  __shared__ int s_unit, s_at;
   __shared__ Walk s_start;
   __shared__ float2 s_final[16];                          // maximum and 1 / sum of a pair's heads
   __shared__ float2 s_sums[16];                           // of this block (clusters)
@@ -334,8 +341,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   griddep_wait();
   griddep_launch_dependents();
 
-  long long unit = 0;                                     // of scores
-  int units = 0, blocks = 0;                              // of the line; that have a stretch
+  long long unit = 0;                                     // tiles ahead of this one, of scores
+  int units = 0, blocks = 0, place_in_line = 0;           // of the line; that have a stretch; of the current tile
   Walk w;
   if constexpr (kCluster) {
     const int pair = block / a.cluster, rank = block - pair * a.cluster, b = pair / a.hkv;
@@ -352,47 +359,52 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     unit = pair * a.pair_tiles + t0;
     __syncthreads();
   } else {
-    // Tiles ahead of each sequence: every thread a run of sequences.
+    // Tiles ahead of each sequence, and sequences that have any: every thread a run of sequences.
     const int run = (a.B + kThreads - 1) / kThreads, from = min(a.B, tid * run), to = min(a.B, from + run);
-    int mine = 0;
+    int2 mine = {0, 0};
     for (int b = from; b < to; ++b) {
       const int rows = rows_of<kStep>(a, b);
-      mine += tiles_of(rows);
+      mine.x += tiles_of(rows);
+      mine.y += rows > 0;
       if (rows < 0 && block == 0) atomicMax(a.status, kStatusBounds);
     }
-    int before = mine;
+    int2 before = mine, all = {0, 0};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += up;
+      const int x = __shfl_up_sync(0xffffffffu, before.x, o), y = __shfl_up_sync(0xffffffffu, before.y, o);
+      if (lane >= o) before.x += x, before.y += y;
     }
     if (lane == 31) s_scan[warp] = before;
-    before -= mine;
+    before.x -= mine.x;
+    before.y -= mine.y;
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < kThreads / 32; ++x) {
-      if (x < warp) before += s_scan[x];
-      units += s_scan[x];
+      const int2 sum = s_scan[x];
+      if (x < warp) before.x += sum.x, before.y += sum.y;
+      all.x += sum.x, all.y += sum.y;
     }
-    units *= a.hkv;
-    before *= a.hkv;
-    mine *= a.hkv;
-    blocks = min(static_cast<int>(gridDim.x), units);
+    units = (all.x + kPair * all.y) * a.hkv;
+    blocks = min(static_cast<int>(gridDim.x), all.x * a.hkv);
     if (block < blocks) {
       const Line line(units, blocks);
-      const int u0 = line.first(block), u1 = line.first(block + 1);
-      if (u0 >= before && u0 < before + mine) {
-        int at = before, b = from, rows = 0;
+      const int u0 = line.first(block), u1 = line.first(block + 1), begin = (before.x + kPair * before.y) * a.hkv;
+      if (u0 >= begin && u0 < begin + (mine.x + kPair * mine.y) * a.hkv) {
+        int at = begin, tiles_ahead = before.x * a.hkv, b = from, rows = 0, tiles = 0;
         for (;; ++b) {
           rows = rows_of<kStep>(a, b);
-          const int all = tiles_of(rows) * a.hkv;
-          if (u0 < at + all) break;
-          at += all;
+          tiles = tiles_of(rows);
+          const int here = tiles > 0 ? (tiles + kPair) * a.hkv : 0;
+          if (u0 < at + here) break;
+          at += here;
+          tiles_ahead += tiles * a.hkv;
         }
-        const int tiles = tiles_of(rows), h = (u0 - at) / tiles;
-        s_start = {b, h, u0 - at - h * tiles, rows, u1 - u0};
+        const int h = (u0 - at) / (tiles + kPair), t = max(0, u0 - at - h * (tiles + kPair) - kPair);
+        at += h * (tiles + kPair) + kPair + t;
+        s_start = {b, h, t, rows, u1 - at};
+        s_unit = tiles_ahead + h * tiles + t;
+        s_at = at;
       }
-      unit = u0;
     }
     // sequences without rows: zeros
     for (int b = block; b < a.B; b += gridDim.x) {
@@ -404,7 +416,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     if (tid == 0) a.stretches[block].blocks = blocks;
     if (block >= blocks) return;
     w = s_start;
-    if (tid == 0) a.stretches[block].begins = static_cast<int>(unit), a.stretches[block].ends = static_cast<int>(unit) + w.left;
+    unit = s_unit;
+    place_in_line = s_at;
+    if (w.left <= 0) {                                    // a part of a pair's beginning only
+      if (tid == 0) {
+        const End none = {-1, block, block, 0};
+        a.stretches[block].begins = a.stretches[block].ends = 0;
+        a.stretches[block].end[0] = a.stretches[block].end[1] = none;
+      }
+      return;
+    }
+    if (tid == 0) a.stretches[block].begins = static_cast<int>(unit);
   }
 
   int stage = 0, phase = 0;
@@ -444,7 +466,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                       value ? &v_map : &k_map, &s_full[stage], x, row % a.c.page, w.h, page);
         advance();
       }
-      next_pair<kStep>(a, w, take);
+      next_pair<kWide, kStep>(a, w, take);
     }
     if (!kCluster) return;
   }
@@ -507,7 +529,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_query);
-      next_pair<kStep>(a, w, take);
+      next_pair<kWide, kStep>(a, w, take);
     }
     if (!kCluster) return;
   }
@@ -548,13 +570,16 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_query_taken);
     }
-    if (!kCluster && tid == 0 && (first_pair || take == w.left)) {
-      const Line line(units, blocks);
-      const int at = static_cast<int>(unit) - w.t;
-      const int first = line.block_of(at);
-      const End end = {pair, first, line.block_of(at + tiles - 1), line.first(first) < at ? 1 : 0};
-      if (first_pair) a.stretches[block].end[0] = end;
-      if (take == w.left) a.stretches[block].end[1] = end;
+    if (!kCluster && tid == 0) {
+      const bool last_pair = w.left - take <= kPair;
+      if (first_pair || last_pair) {
+        const Line line(units, blocks);
+        const int at = place_in_line - w.t, first = line.block_of(at);
+        const End end = {pair, first, line.block_of(at + tiles - 1), line.first(first) < at - kPair ? 1 : 0};
+        if (first_pair) a.stretches[block].end[0] = end;
+        if (last_pair) a.stretches[block].end[1] = end, a.stretches[block].ends = static_cast<int>(unit) + take;
+      }
+      place_in_line += take + kPair;
     }
 
     float m[kHeads], l[kHeads], o[D / 8][4];
@@ -770,7 +795,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     }
     if constexpr (kCluster) break;
     first_pair = false;
-    next_pair<kStep>(a, w, take);
+    next_pair<kWide, kStep>(a, w, take);
   }
   if constexpr (kCluster) {
     // Every block adds the heads' maxima and sums, the first one the columns too: a warp a share of them.

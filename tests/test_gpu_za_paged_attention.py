@@ -77,6 +77,17 @@ def test_pairs_cut_between_most_blocks(lengths, G, D):
     _attend(lengths, 1, G, D, 64, seed=G, weights=G % 2 == 1)
 
 
+@pytest.mark.parametrize("G,D", [(2, 128), (16, 128), (3, 64)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_many_short_pairs_beside_long_ones(G, D, weights):
+    """Pairs of a tile each, whose beginnings are most of what a block has, ahead of, behind and between long ones; stretches that lie
+    within a pair's beginning."""
+    _attend([3000] * 6 + [1, 64, 0, 65] * 15 + [2500], 2, G, D, 64, seed=G, weights=weights)
+    _attend([5] * 40 + [9000] + [0, 70] * 20, 5, G, D, 16, seed=G + 1, weights=weights, order="rows")
+    _attend([1100], 1, G, D, 64, seed=G + 2, weights=weights)
+    _attend([9, 0, 9000, 9], 1, G, D, 64, seed=G + 3, weights=weights)
+
+
 def test_strides_and_shared_pages():
     """Pools that are every other page and a part of the heads of larger ones, a table that is a part of a wider one, two
     sequences that share their first pages."""
