@@ -1,5 +1,6 @@
 // Internal launch functions shared by the translation units of libcdeep.so.
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdlib>
 #include <cuda_runtime.h>
@@ -45,6 +46,34 @@ inline cudaError_t allow_smem(int bytes) {
   return static_cast<cudaError_t>(limit.raise(device, bytes, [](int n) {
     return static_cast<int>(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, n));
   }));
+}
+
+// Clusters of up to 16 blocks of a kernel that run at the same time on the current device (a cluster lies within a part of it, so that they
+// can be fewer than the SMs have room for). `bytes` of dynamic shared memory are the same in all calls; the driver is asked once for
+// each device and size.
+template <auto kKernel>
+inline int clusters_side_by_side(int blocks, int threads, int bytes) {
+  constexpr int kDevices = 64, kUnlimited = 1 << 30;
+  static std::atomic<int> known[kDevices][17];            // one more than the answer
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= kDevices || blocks > 16) return kUnlimited;
+  if (const int k = known[device][blocks].load(std::memory_order_relaxed)) return k - 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (allow_smem<kKernel>(bytes) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();                                   // nothing is known: no limit
+    return kUnlimited;
+  }
+  known[device][blocks].store(n + 1, std::memory_order_relaxed);
+  return n;
 }
 
 size_t route_workspace_bytes(int T, int E);

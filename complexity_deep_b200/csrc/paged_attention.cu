@@ -1001,17 +1001,30 @@ __global__ void __launch_bounds__(kFinishThreads) paged_finish_kernel(const Args
   }
 }
 
+// What a step needs of an SM is the same.
+int clusters_of_pairs(int D, bool wide, int blocks) {
+#define CDEEP_FIT(DD, WIDE)  \
+  if (D == DD && wide == WIDE) return clusters_side_by_side<paged_attention_kernel<DD, WIDE, false, true>>(blocks, kThreads, smem_bytes(DD, WIDE));
+  CDEEP_FIT(64, false) CDEEP_FIT(64, true) CDEEP_FIT(128, false) CDEEP_FIT(128, true)
+#undef CDEEP_FIT
+  return 1 << 30;
+}
+
 // Blocks of a pair where short caches take clusters, else 0: as many as give every block an SM to itself, twice as many where they
 // would have more than eight tiles and two fit an SM; up to 16 tiles a block. us, cold L2, events included, line / clusters of 1 / 2 / 4 / 8,
 // 8 heads of 2 x 128: 1 x 512 rows 15 / 16 / 13 / 12 / 12, 1 x 4 096 26 / 55 / 33 / 23 / 16, 4 x 1 024 20 / 21 / 16 / 14 / 16, 4 x 4 096
 // 30 / 55 / 35 / 27 / 27, 8 x 512 18 / 16 / 14 / 16 / 23, 8 x 2 048 30 / 33 / 27 / 25 / 33, 16 x 1 024 30 / 25 / 25 / 31, 16 x 2 048
 // 42 / 39 / 39 / 43, 32 x 256 22 / 19 / 24, 32 x 1 024 42 / 37 / 43, 64 x 128 22 / 23, 64 x 512 42 / 41; with weights, lengths between a
 // half and all: 8 x 1 024 24 / 27 / 23 / 21 / 27, 32 x 1 024 40 / 39 / 45.
-int cluster_of(long long pairs, long long tiles, int fit) {
+// Clusters that do not fit side by side (they lie within a part of the GPU, and 16 heads of 128 have an SM to a block) are halved: 16
+// clusters of eight took two turns, 4 x 1 000 rows, 4 x 16 x 128, 20.3, of four 11.4.
+int cluster_of(long long pairs, long long tiles, int D, bool wide) {
+  const int fit = blocks_per_sm(D, wide);
   const long long sms = current_sm_count();
   int blocks = 1;
   while (blocks < kMostCluster && 2 * blocks * pairs <= sms && 2 * blocks <= tiles) blocks *= 2;
   if (blocks < kMostCluster && 2 * blocks * pairs <= fit * sms && tiles > kClusterTiles / 2 * blocks) blocks *= 2;
+  while (blocks > 1 && pairs > clusters_of_pairs(D, wide, blocks)) blocks /= 2;
   return blocks * pairs <= fit * sms && (tiles + blocks - 1) / blocks <= kClusterTiles ? blocks : 0;
 }
 
@@ -1023,7 +1036,7 @@ struct Layout {
 };
 Layout layout(int B, int hkv, int G, int D, int page, int width, bool weights) {
   Layout l = {};
-  l.cluster = cluster_of(static_cast<long long>(B) * hkv, (static_cast<long long>(width) * page + kTile - 1) / kTile, blocks_per_sm(D, G > 8));
+  l.cluster = cluster_of(static_cast<long long>(B) * hkv, (static_cast<long long>(width) * page + kTile - 1) / kTile, D, G > 8);
   auto take = [&](size_t n) {
     const size_t at = l.bytes;
     l.bytes += (n + 255) / 256 * 256;

@@ -36,7 +36,7 @@ constexpr int kList = 512;                 // entries compared with one another
 constexpr int kFew = 256;                  // the largest k that takes the bound
 constexpr int kMany = 2048;                // tokens that a larger top-k leaves in a block, as a list
 constexpr int kMostBlocks = 8;             // of a row: the largest cluster that every device takes
-constexpr int kSliceBytes = 128 * 1024;    // of a row in a block: 2^16 tokens at most; 2^18 numbers of 32 bits are eight blocks
+constexpr int kSliceBytes = 160 * 1024;    // of a row in a block, beside what Shared takes: 2^18 numbers of 32 bits are eight blocks
 using u64 = unsigned long long;
 constexpr u64 kOne = 1ull << 44;
 
@@ -116,6 +116,8 @@ struct Shared {
   unsigned counts[kMostBlocks], opens;
   int bin;
 };
+
+static_assert((sizeof(Shared<1024>) + 15) / 16 * 16 + kSliceBytes + 32 * 16 <= 232448, "a block's share and what it is taken apart with");
 
 template <typename T, int kThreads>
 struct Row {
@@ -825,6 +827,11 @@ cudaError_t launch_one(const void* logits, long long ld, int B, int V, const cd_
   int blocks = 1;
   while (static_cast<long long>(V) * sizeof(T) > static_cast<long long>(blocks) * kSliceBytes) blocks *= 2;
   while (blocks < kMostBlocks && 2LL * blocks * B <= current_sm_count() && V / (2 * blocks) >= 4096) blocks *= 2;
+  // 1 024 threads are an SM's: clusters of them that would have to wait for one another are halved, where halves have room for the row. us, 37 x 100 000
+  // with a top-k of 50 19 -> 13, its nucleus 65 -> 44, nucleus of 18 x 250 000 116 -> 74.
+  while (blocks > 1 && V / blocks > 16384 && B > clusters_side_by_side<sample_tokens_kernel<T, 1024>>(blocks, 1024, 1024) &&
+         2 * static_cast<long long>(V) * sizeof(T) <= static_cast<long long>(blocks) * kSliceBytes)
+    blocks /= 2;
   const T* x = static_cast<const T*>(logits);
   long long* to = reinterpret_cast<long long*>(ids);
   return V / blocks > 16384 ? launch_blocks<T, 1024>(blocks, x, ld, B, V, p, to, probs, stream)

@@ -10,14 +10,14 @@ import paged_cases as cases
 pytestmark = pytest.mark.gpu
 
 
-def _check(x, u, t=1.0, k=0, p=1.0, m=0.0):
+def _check(x, u, t=1.0, k=0, p=1.0, m=0.0, rows=None):
     from complexity_deep_b200 import ops
     rules = [r.cuda() if isinstance(r, torch.Tensor) else r for r in (t, k, p, m)]
     ids, probs = ops.sample_tokens(x.cuda(), u.cuda(), *rules)
     ids2, probs2 = ops.sample_tokens(x.cuda(), u.cuda(), *rules)
     assert torch.equal(ids, ids2) and torch.equal(probs, probs2)
     f32 = lambda v, i: float(v[i] if isinstance(v, torch.Tensor) else torch.tensor(v, dtype=torch.float32))  # noqa: E731
-    for i in range(x.shape[0]):
+    for i in range(x.shape[0]) if rows is None else rows:
         want, prob = cases.sample(x[i], float(u[i]), f32(t, i), int(k[i] if isinstance(k, torch.Tensor) else k), f32(p, i), f32(m, i))
         assert int(ids[i]) == want, (i, int(ids[i]), want)
         assert abs(float(probs[i]) - prob) <= 2.0 ** -23 * prob + 1e-12, (i, float(probs[i]), prob)
@@ -66,6 +66,15 @@ def test_largest_vocabulary():
     _check(x, u, 1.0, 0, 0.9, 0.0)
     _check(x, u, 1.0, 300, 0.9, 0.0)
     _check(torch.zeros(1, 1 << 18), torch.tensor([0.75]), 1.0, 0, 1.0, 0.0)    # the largest sum that there is
+
+
+@pytest.mark.parametrize("B,V,dtype", [(75, 40960, torch.float32), (75, 40961, torch.float32), (75, 81920, torch.bfloat16),
+                                       (38, 163840, torch.bfloat16), (37, 70000, torch.bfloat16), (20, 200000, torch.bfloat16)])
+def test_shares_of_a_row(B, V, dtype):
+    """The largest share that a block takes and one token more; rows whose clusters would not run at the same time."""
+    x, u = _inputs(B, V, dtype, B)
+    for rules in ((1.0, 0, 0.9, 0.0), (1.0, 3000, 0.99, 0.001), (0.8, 50, 0.9, 0.0)):
+        _check(x, u, *rules, rows=(0, B // 2, B - 1))
 
 
 def test_rules_by_row():
