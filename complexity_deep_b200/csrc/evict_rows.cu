@@ -387,11 +387,14 @@ cudaError_t launch_one(const Args& a, int pairs, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kKernel, a);
 }
 
-// Blocks of a pair: more than one where there are SMs without, and 4 096 rows, or 512 that may move, for each.
+// Blocks of a pair: more than one where there are SMs without, and 4 096 rows, or 512 that may move, for each, and all clusters run at
+// the same time (of the blocks of 1 024 threads that are likely then, an SM has one). 16 pairs of 18 830 rows to 1 176 with eight blocks
+// each, of which not all 16 run together, 51 us, with four 29; 34 of them 49 and 37.
 int blocks_of(long long pairs, int rows, int keep) {
   const int most = rows - keep < keep ? rows - keep : keep;
   int blocks = 1;
   while (blocks < kMostBlocks && 2 * blocks * pairs <= current_sm_count() && (most >= 512 * blocks || rows >= 4096 * blocks)) blocks *= 2;
+  while (blocks > 1 && pairs > clusters_side_by_side<evict_rows_kernel<1024, true>>(blocks, 1024, 32 * 1024)) blocks /= 2;
   return blocks;
 }
 int share_of(int rows, int blocks) { return ((rows + blocks - 1) / blocks + 31) / 32 * 32; }
@@ -431,10 +434,11 @@ cudaError_t launch_evict_rows(const cd_paged& c, const cd_evict& e, int layers, 
   // 1024x4 37. With one block a pair, 128, 256 and 1 024 threads: 128 of 2 304 to 2 048 43, 29, 23; 160 of 3 000 to 2 048 100, 61, 55;
   // 192 of 1 100 to 1 024 23, 18, 29; 192 of 4 096 to 2 048 154, 90, 72; 256 of 2 304 49, 35, 37; 512 57, 47, 68; 512 of 3 300 144,
   // 106, 125; 512 of 8 192 to 4 096 366, 246, 254; 1 024 of 2 304 80, 82, 115; 768 of 1 100 33, 37, 70; 640 of 3 300 156, 160, 154; 640
-  // of 4 096 197, 201, 182.
+  // of 4 096 197, 201, 182; 3 072 of 4 096 705, 698, 757; 6 144 of 2 304 395, 376, 637 (a table may have room for
+  // more rows than there are, which smaller blocks mind less).
   const long long grid = static_cast<long long>(pairs) * a.blocks, sms = current_sm_count();
   if (grid > 4 * sms && a.share <= 2560) return launch_one<128, true>(a, pairs, stream);
-  if (grid <= 4 * sms && a.share <= (grid <= sms ? 511 : 4000)) return launch_one<256, true>(a, pairs, stream);
+  if (a.share <= (grid <= sms ? 511 : grid <= 4 * sms ? 4000 : 8192)) return launch_one<256, true>(a, pairs, stream);
   return a.share <= kHeldRows ? launch_one<1024, true>(a, pairs, stream) : launch_one<1024, false>(a, pairs, stream);
 }
 

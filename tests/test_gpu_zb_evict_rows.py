@@ -83,9 +83,9 @@ def test_several_blocks_a_pair(rows, keep, ties):
     _run([rows - 7], 3, 16, 32, keep, keep // 3, seed=keep, ties=ties, in_place=not ties, width=-(-rows // 32) + 9)
 
 
-@pytest.mark.parametrize("pairs,rows", [(149, 400), (149, 3990), (149, 4100), (600, 200), (600, 2600), (600, 60)])
+@pytest.mark.parametrize("pairs,rows", [(16, 9000), (36, 5000), (149, 400), (149, 3990), (149, 4100), (600, 200), (600, 2600), (600, 60)])
 def test_many_pairs(pairs, rows):
-    """More pairs than SMs, and than four an SM: blocks of 128, 256 and 1 024 threads."""
+    """Pairs whose clusters would not all run together, more pairs than SMs, and than four an SM: blocks of 128, 256 and 1 024 threads."""
     from complexity_deep_b200 import ops
     g = torch.Generator().manual_seed(rows)
     width = -(-rows // 16)
