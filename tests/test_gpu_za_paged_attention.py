@@ -85,6 +85,7 @@ def test_many_short_pairs_beside_long_ones(G, D, weights):
     _attend([3000] * 6 + [1, 64, 0, 65] * 15 + [2500], 2, G, D, 64, seed=G, weights=weights)
     _attend([5] * 40 + [9000] + [0, 70] * 20, 5, G, D, 16, seed=G + 1, weights=weights, order="rows")
     _attend([1100], 1, G, D, 64, seed=G + 2, weights=weights)
+    _attend([(53 * i) % 211 * (i % 5 > 0) for i in range(450)], 2, G, D, 16, seed=G + 4, weights=weights)     # several sequences a thread
     _attend([9, 0, 9000, 9], 1, G, D, 64, seed=G + 3, weights=weights)
 
 
