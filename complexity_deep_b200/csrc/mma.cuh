@@ -37,5 +37,12 @@ __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t& hi, uin
   hi = bf_pack(v0, v1);
   lo = bf_pack(v0 - bf_lo(hi), v1 - bf_hi(hi));
 }
+// v0, v1 as three bf16 pairs hi + lo + rest: all of their 24 significant bits, down to the smallest bf16
+__device__ __forceinline__ void split_all(float v0, float v1, uint32_t& hi, uint32_t& lo, uint32_t& rest) {
+  hi = bf_pack(v0, v1);
+  const float r0 = v0 - bf_lo(hi), r1 = v1 - bf_hi(hi);
+  lo = bf_pack(r0, r1);
+  rest = bf_pack(r0 - bf_lo(lo), r1 - bf_hi(lo));
+}
 
 }  // namespace cdeep

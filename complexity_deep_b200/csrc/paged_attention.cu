@@ -5,8 +5,9 @@
 //
 // for the G query heads g of a KV head: every cached row is read once for all of them, so the read (4 D bytes a row and head) is
 // the bound, and G only has to stay out of its way. Hence matrix instructions (m16n8k16): the query heads are the 16 rows of one
-// operand. Up to eight heads leave half of them free, which hold what bf16 cuts off: q and p enter as two bf16 numbers (16
-// significant bits) at no cost. More heads take two products instead.
+// operand. Keys and values are bf16; q (of a step) and p have 32 bits and enter as three bf16 numbers, which hold all 24 of their
+// significant ones. Up to eight heads leave half of the rows free: the first two numbers share a product, the third takes one of its
+// own. More heads take three. A q that comes as bf16 is one number.
 //
 // Work is cut into tiles of 64 rows; all tiles of all (sequence, KV head) pairs stand in one line, of which every block takes an equal
 // stretch, whatever the lengths are (a pair's beginning counts as a few tiles: pair_units). A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
@@ -48,12 +49,13 @@ __host__ __device__ constexpr int stage_bytes(int D) { return 2 * kTile * D * 2;
 // floats of a lane that a warp hands over: its columns of each head it holds
 __host__ __device__ constexpr int lane_floats(int D, bool wide) { return D / 8 * (wide ? 4 : 2); }
 __host__ __device__ constexpr int merge_bytes(int D, bool wide) { return kSlots * 32 * (lane_floats(D, wide) + 4) * 4; }
-// operand fragments of a pair's query heads, then the new row's key and value
-__host__ __device__ constexpr int query_bytes(int D, bool wide) { return D / 16 * 32 * 16 * (wide ? 2 : 1) + 2 * D * 2; }
+// operand fragments of a pair's query heads (the first two numbers), the new row's key and value, the fragments' third numbers
+__host__ __device__ constexpr int query_bytes(int D, bool wide) { return D / 16 * 32 * (16 + 8) * (wide ? 2 : 1) + 2 * D * 2; }
 // Two blocks an SM (113 KB each): one computes while the other starts a pair or ends one. 16 heads of 128 leave room for one.
 __host__ __device__ constexpr int blocks_per_sm(int D, bool wide) { return wide && D == 128 ? 1 : 2; }
 __host__ __device__ constexpr int stages_of(int D, bool wide) {
-  return (232448 / blocks_per_sm(D, wide) - 1024 * 2 - 512 - merge_bytes(D, wide) - query_bytes(D, wide)) / stage_bytes(D);
+  // an SM's 228 KB, of which each block takes 1 KB for the system, up to 1 KB for the ring's alignment, 512 bytes outside of it
+  return (233472 / blocks_per_sm(D, wide) - 1024 * 2 - 512 - merge_bytes(D, wide) - query_bytes(D, wide)) / stage_bytes(D);
 }
 __host__ __device__ constexpr int smem_bytes(int D, bool wide) {
   return 1024 + stages_of(D, wide) * stage_bytes(D) + merge_bytes(D, wide) + query_bytes(D, wide);
@@ -323,6 +325,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   float* s_merge = reinterpret_cast<float*>(ring + kStages * stage_bytes(D));
   uint4* s_heads = reinterpret_cast<uint4*>(ring + kStages * stage_bytes(D) + merge_bytes(D, kWide));
   bf16* s_new = reinterpret_cast<bf16*>(s_heads + D / 16 * 32 * (kWide ? 2 : 1));
+  uint2* s_rest = reinterpret_cast<uint2*>(s_new + 2 * D);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int block = blockIdx.x;
 
@@ -480,26 +483,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       NewRow<D> row;
       if (kStep && last_tile)
         row.load(a, q + static_cast<long long>(a.hkv * a.G + w.h) * D, q + static_cast<long long>(a.hkv * (a.G + 1) + w.h) * D, pos, lane);
-      // what bf16 holds of the heads and what it cuts off
-      uint4 part[D / 16][kWide ? 2 : 1];
-      float v[D / 16][4];
-      load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0) * D, g0 < a.G, pos, lane, v);
+      float v[kHeads][D / 16][4];
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        uint32_t hi[2], lo[2];
-        split_pair(v[k][0], v[k][1], hi[0], lo[0]);
-        split_pair(v[k][2], v[k][3], hi[1], lo[1]);
-        part[k][0] = kWide ? make_uint4(hi[0], 0, hi[1], 0) : make_uint4(hi[0], lo[0], hi[1], lo[1]);
-        if constexpr (kWide) part[k][1] = make_uint4(lo[0], 0, lo[1], 0);
-      }
-      if constexpr (kWide) {
-        load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0 + 8) * D, g0 + 8 < a.G, pos, lane, v);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          split_pair(v[k][0], v[k][1], part[k][0].y, part[k][1].y);
-          split_pair(v[k][2], v[k][3], part[k][0].w, part[k][1].w);
-        }
-      }
+      for (int i = 0; i < kHeads; ++i)
+        load_head<D, kStep>(a, q + static_cast<long long>(w.h * a.G + g0 + 8 * i) * D, g0 + 8 * i < a.G, pos, lane, v[i]);
       bf16 key[D / 32];
       if (kStep && last_tile) {
         row.key(a, key);
@@ -517,8 +504,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       if (!mbar_wait(&s_query_taken, turn ^ 1, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
+        uint32_t hi[kHeads][2], lo[kHeads][2], rest[kHeads][2];
 #pragma unroll
-        for (int i = 0; i < (kWide ? 2 : 1); ++i) s_heads[(k * (kWide ? 2 : 1) + i) * 32 + lane] = part[k][i];
+        for (int i = 0; i < kHeads; ++i) {
+          split_all(v[i][k][0], v[i][k][1], hi[i][0], lo[i][0], rest[i][0]);
+          split_all(v[i][k][2], v[i][k][3], hi[i][1], lo[i][1], rest[i][1]);
+        }
+        if constexpr (kWide) {
+          s_heads[2 * k * 32 + lane] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
+          s_heads[(2 * k + 1) * 32 + lane] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
+        } else {
+          s_heads[k * 32 + lane] = make_uint4(hi[0][0], lo[0][0], hi[0][1], lo[0][1]);
+        }
+        if constexpr (kStep) {
+#pragma unroll
+          for (int i = 0; i < kHeads; ++i) s_rest[(kHeads * k + i) * 32 + lane] = make_uint2(rest[i][0], rest[i][1]);
+        }
       }
       if (kStep && last_tile) {
 #pragma unroll
@@ -568,7 +569,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_query_taken);
+      if (!kStep && lane == 0) mbar_arrive(&s_query_taken);  // the third numbers of a step are read with every tile
     }
     if (!kCluster && tid == 0) {
       const bool last_pair = w.left - take <= kPair;
@@ -620,9 +621,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             mma16816(s[0], ql[k], kb[0], kb[1]);
             mma16816(s[1], ql[k], kb[2], kb[3]);
           }
+          if constexpr (kStep) {
+            const uint2 r = s_rest[kHeads * k * 32 + lane], r2 = kWide ? s_rest[(kHeads * k + 1) * 32 + lane] : make_uint2(0, 0);
+            const uint32_t rest[4] = {r.x, r2.x, r.y, r2.y};
+            mma16816(s[0], rest, kb[0], kb[1]);
+            mma16816(s[1], rest, kb[2], kb[3]);
+          }
         }
         // p of head i of this lane at keys col + {0, 1, 8, 9}
-        uint32_t ph[4], pl[4];
+        uint32_t ph[4], pl[4], pr[4] = {};
 #pragma unroll
         for (int i = 0; i < kHeads; ++i) {
           float x[4];
@@ -659,8 +666,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             l[i] += x[e];
           }
           uint32_t hi[2], lo[2];
-          split_pair(x[0], x[1], hi[0], lo[0]);
-          split_pair(x[2], x[3], hi[1], lo[1]);
+          split_all(x[0], x[1], hi[0], lo[0], pr[i]);
+          split_all(x[2], x[3], hi[1], lo[1], pr[2 + i]);
           if constexpr (kWide) {
             ph[i] = hi[0];
             ph[2 + i] = hi[1];
@@ -696,12 +703,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             mma16816(o[2 * j], pl, vb[0], vb[1]);
             mma16816(o[2 * j + 1], pl, vb[2], vb[3]);
           }
+          mma16816(o[2 * j], pr, vb[0], vb[1]);
+          mma16816(o[2 * j + 1], pr, vb[2], vb[3]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_empty[stage]);
       advance();
     }
+    if (kStep && take > 0 && lane == 0) mbar_arrive(&s_query_taken);
 
     // The four warps' sums meet in the first, lane by lane (all hold the same heads and columns).
     float f[kFloats];
