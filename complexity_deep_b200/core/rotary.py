@@ -12,12 +12,17 @@ import torch
 import torch.nn as nn
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class RotaryEmbedding(nn.Module):
     def __init__(self, dim: int, max_seq_len: int = 2048, theta: float = 10000.0):
         super().__init__()
         self.dim, self.max_seq_len, self.theta = dim, max_seq_len, theta
         exponents = torch.arange(0, dim, 2).float() / dim
         self.register_buffer("inv_freq", 1.0 / (theta ** exponents))
+        self._captured = []               # tables whose addresses CUDA graphs hold
         self._build_cache(max_seq_len)
 
     def _build_cache(self, seq_len: int) -> None:
@@ -38,6 +43,9 @@ class RotaryEmbedding(nn.Module):
 
         ``module.to(bfloat16)`` also casts the cached tables; they are then rebuilt in fp32
         from ``inv_freq`` so the kernel always reads full-precision angles.
+
+        A CUDA graph keeps the addresses that its launches were captured with and nothing alive: tables
+        handed out during a capture stay as long as the module, also when longer ones take their place.
         """
         if seq_len > self.max_seq_len or self.cos_cached.dtype != torch.float32:
             if self.inv_freq.dtype != torch.float32:
@@ -48,6 +56,8 @@ class RotaryEmbedding(nn.Module):
                 # rebuild the tables on every step
                 self.max_seq_len = 1 << (seq_len - 1).bit_length()
             self._build_cache(self.max_seq_len)
+        if _capturing(self.cos_cached) and not any(cos is self.cos_cached for cos, _ in self._captured):
+            self._captured.append((self.cos_cached, self.sin_cached))
         return self.cos_cached, self.sin_cached
 
 
