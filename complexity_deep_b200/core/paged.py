@@ -81,24 +81,40 @@ class PagedKVCache:
     def _send(self) -> None:
         self.table.copy_(self._table, non_blocking=True)     # from pageable memory: the host's copy is free when the call returns
 
-    def add(self, past_key_values, row: int = 0) -> int:
-        """Takes over the cache of sequence `row` of a prompt (list of (k, v) [B, kv heads, P, D]) and returns the slot."""
-        rows = past_key_values[0][0].shape[2]
+    def room_for(self, rows: int) -> int:
+        """The slot that a prompt of so many tokens gets; raises if there is no slot, row or page for it."""
         if -1 not in self._length:
             raise RuntimeError(f"all {self.slots} slots are in use")
         if not 1 <= rows <= self.max_rows or rows > self.max_positions:
             raise ValueError(f"{rows} tokens do not fit sequences of {self.max_rows} rows")
-        slot = self._length.index(-1)
+        count = -(-rows // self.page)
+        if count > len(self._free):
+            raise RuntimeError(f"no page left: {count} wanted, {len(self._free)} of {self.pages} free")
+        return self._length.index(-1)
+
+    def add(self, past_key_values, row: int = 0) -> int:
+        """Takes over the cache of sequence `row` of a prompt (list of (k, v) [B, kv heads, P, D]) and returns the slot.  What does not
+        fit is refused before anything is changed."""
+        layers, _, kv_heads, _, dim = self.k.shape
+        B, _, rows, _ = shape = past_key_values[0][0].shape
+        if len(past_key_values) != layers or not -B <= row < B or any(t.shape != (B, kv_heads, rows, dim) for p in past_key_values for t in p):
+            raise ValueError(f"expected sequence {row} of {layers} layers of [B, {kv_heads}, rows, {dim}], the first of "
+                             f"{len(past_key_values)} is {list(shape)}")
+        slot = self.room_for(rows)
         count = -(-rows // self.page)
         self._take(slot, count)
-        ids = torch.tensor(self._pages[slot], device=self.k.device)
-        for i, pair in enumerate(past_key_values):
-            for pool, t in zip((self.k, self.v), pair):
-                t = torch.nn.functional.pad(t[row], (0, 0, 0, count * self.page - rows))
-                pool[i, ids] = t.unflatten(1, (count, self.page)).transpose(0, 1)
-        if self.weights is not None:
-            self.weights[:, slot, :, :rows] = 0.0
-            self.row_positions[:, slot, :, :rows] = torch.arange(rows, dtype=torch.int32, device=self.k.device)
+        try:
+            ids = torch.tensor(self._pages[slot], device=self.k.device)
+            for i, pair in enumerate(past_key_values):
+                for pool, t in zip((self.k, self.v), pair):
+                    t = torch.nn.functional.pad(t[row], (0, 0, 0, count * self.page - rows))
+                    pool[i, ids] = t.unflatten(1, (count, self.page)).transpose(0, 1)
+            if self.weights is not None:
+                self.weights[:, slot, :, :rows] = 0.0
+                self.row_positions[:, slot, :, :rows] = torch.arange(rows, dtype=torch.int32, device=self.k.device)
+        except BaseException:                             # no memory for the copies
+            self._give_back(slot, 0)
+            raise
         self._length[slot] = self._position[slot] = rows
         self.lengths[slot] = self.positions[slot] = rows
         self.live[slot] = 1

@@ -61,12 +61,15 @@ class PagedDecoder:
     def add(self, prompt_ids: torch.Tensor, uniform: float = 0.0, temperature: float = 1.0, top_k: int = 50, top_p: float = 0.9,
             min_p: float = 0.0) -> Tuple[int, torch.Tensor]:
         """Runs a prompt [P] and gives it a slot; its rules hold until ``release``.  Returns the slot and the first token drawn
-        behind the prompt [1], by `uniform` (0 <= uniform < 1)."""
+        behind the prompt [1], by `uniform` (0 <= uniform < 1).  A prompt without a slot, rows or pages for it and rules that are no
+        numbers are refused before the prompt runs."""
+        self.cache.room_for(prompt_ids.numel())
+        rules = [(self.temperature, float(temperature)), (self.top_k, max(0, min(int(top_k), 2 ** 31 - 1))), (self.top_p, float(top_p)),
+                 (self.min_p, float(min_p)), (self.uniform, float(uniform))]
         with torch.no_grad():
             out = self.model(prompt_ids.view(1, -1).to(self.ids.device), use_cache=True)
         slot = self.cache.add(out.past_key_values)
-        for rule, value in ((self.temperature, temperature), (self.top_k, top_k), (self.top_p, top_p), (self.min_p, min_p),
-                            (self.uniform, uniform)):
+        for rule, value in rules:
             rule[slot] = value
         one = slice(slot, slot + 1)
         first, _ = ops.sample_tokens(out.logits[:, -1], self.uniform[one], self.temperature[one], self.top_k[one], self.top_p[one],
