@@ -9,7 +9,7 @@ back by them.
 """
 from __future__ import annotations
 
-from typing import List
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -164,15 +164,26 @@ class PagedKVCache:
         self.advance_device()
         self.advance_host()
 
-    def evict(self, keep: int, recent: int) -> None:
-        """Cuts every sequence of more than `keep` rows back to `keep` per layer and KV head: the last `recent` tokens and the rows of
-        largest weight (``ops.evict_rows_``).  The pages behind them are free afterwards."""
+    def evict(self, keep: int, recent: int, slots: Optional[Sequence[int]] = None) -> None:
+        """Cuts every sequence (of those slots, where they are given) of more than `keep` rows back to `keep` per layer and KV head: the
+        last `recent` tokens and the rows of largest weight (``ops.evict_rows_``).  The pages behind them are free afterwards.  Weights
+        are those of the steps so far: a prompt's rows come with none."""
         if self.weights is None:
             raise RuntimeError("evict needs a cache with statistics")
-        ops.evict_rows_(self.k, self.v, self.table, self.lengths, self.positions, self.weights, self.row_positions, keep, recent)
-        self.lengths.clamp_(max=keep)
-        for slot, n in enumerate(self._length):
-            if n > keep:
+        lengths = self.lengths
+        chosen = range(self.slots) if slots is None else slots
+        if slots is not None:                             # the others look as if they were not in use
+            these = torch.zeros(self.slots, dtype=torch.bool)
+            these[list(slots)] = True
+            these = these.to(lengths.device)
+            lengths = torch.where(these, lengths, -1)
+        ops.evict_rows_(self.k, self.v, self.table, lengths, self.positions, self.weights, self.row_positions, keep, recent)
+        if slots is None:
+            self.lengths.clamp_(max=keep)
+        else:
+            self.lengths.copy_(torch.where(these, self.lengths.clamp(max=keep), self.lengths))
+        for slot in chosen:
+            if self._length[slot] > keep:
                 self._length[slot] = keep
                 self._give_back(slot, -(-keep // self.page))
         self._send()

@@ -20,17 +20,22 @@ class PagedDecoder:
         ids, probs = dec.step(torch.rand(32, device="cuda"))     # [slots] each, overwritten by the next step
         dec.release(slot)
 
-    keep: sequences are cut back to that many rows when one of them has max_rows (0: it then raises).  Entries of slots that
-    are not in use mean nothing."""
+    keep: a sequence is cut back to that many rows when it has `cut` rows (max_rows unless given; keep 0: a sequence with max_rows
+    raises).  Which rows stay goes by the attention that steps have paid them, and a prompt's rows come without any: one of more
+    than `keep` tokens is first cut when it has cut - keep more, as far as max_rows goes; one of max_rows tokens is cut before its first
+    step, to its first rows and the `recent` newest.  Entries of slots that are not in use mean nothing."""
 
     def __init__(self, model, slots: int, pages: int, page: int = 64, max_rows: int = 2048, max_positions: Optional[int] = None,
-                 keep: int = 0, recent: int = 0, warmup: int = 2) -> None:
+                 keep: int = 0, recent: int = 0, warmup: int = 2, cut: Optional[int] = None) -> None:
         if keep and not (0 <= recent <= keep < max_rows):
             raise ValueError("expected 0 <= recent <= keep < max_rows")
+        if cut is not None and not 0 < keep < cut <= max_rows:
+            raise ValueError("expected 0 < keep < cut <= max_rows")
         device = next(model.parameters()).device
         if device.type != "cuda":
             raise RuntimeError("PagedDecoder needs the model on a CUDA device")
-        self.model, self.keep, self.recent = model, keep, recent
+        self.model, self.keep, self.recent, self.cut = model, keep, recent, cut or max_rows
+        self._limit = [self.cut] * slots      # rows at which a slot's sequence is cut
         self.cache = model.make_paged_cache(slots, pages, page, max_rows, max_positions, statistics=keep > 0)
         on = dict(device=device)
         self.ids = torch.zeros(slots, 1, dtype=torch.int64, **on)
@@ -69,6 +74,7 @@ class PagedDecoder:
         with torch.no_grad():
             out = self.model(prompt_ids.view(1, -1).to(self.ids.device), use_cache=True)
         slot = self.cache.add(out.past_key_values)
+        self._limit[slot] = min(self.cache.max_rows, max(self.keep, prompt_ids.numel()) + self.cut - self.keep)
         for rule, value in rules:
             rule[slot] = value
         one = slice(slot, slot + 1)
@@ -79,8 +85,11 @@ class PagedDecoder:
 
     def step(self, uniform: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """The next token of every sequence in use: (ids [slots], their probabilities [slots]), from uniform numbers [slots]."""
-        if self.keep and self.cache.full():
-            self.cache.evict(self.keep, self.recent)
+        due = [slot for slot, limit in enumerate(self._limit) if self.cache.length(slot) >= limit] if self.keep else []
+        if due:
+            self.cache.evict(self.keep, self.recent, due)
+            for slot in due:
+                self._limit[slot] = self.cut
         self.cache.reserve()
         self.uniform.copy_(uniform, non_blocking=True)
         self.graph.replay()
@@ -95,19 +104,25 @@ def paged_generate(model, prompts: Sequence[torch.Tensor], max_new_tokens: int =
                    top_p: float = 0.9, min_p: float = 0.0, eos_token_id: Optional[int] = None, page: int = 64, keep: int = 0,
                    recent: int = 0, seed: Optional[int] = None) -> List[List[int]]:
     """Continues prompts of any lengths side by side; each stops at the end token (the config's, unless given) or after
-    `max_new_tokens`.  temperature 0: greedy.  keep: sequences are cut back to that many rows whenever one has an eighth
-    (at least a page) more.  Returns prompt and continuation of each."""
+    `max_new_tokens`.  temperature 0: greedy.  keep: a sequence is cut back to that many rows whenever it has an eighth (at least a
+    page) more, one with a longer prompt for the first time when it has as many more than the prompt.  Returns prompt and
+    continuation of each."""
     if not prompts or min(len(p) for p in prompts) < 1:
         raise ValueError("paged_generate needs prompts of at least one token")
     if max_new_tokens < 1:
         return [list(map(int, p)) for p in prompts]
     eos = getattr(model.config, "eos_token_id", None) if eos_token_id is None else eos_token_id
     device = next(model.parameters()).device
-    longest = max(len(p) for p in prompts)
-    last = longest + max_new_tokens
-    max_rows = max(longest, min(last, keep + max(page, keep // 8))) if keep else last
-    dec = PagedDecoder(model, len(prompts), len(prompts) * -(-max_rows // page), page, max_rows, last, keep if keep < max_rows else 0,
-                       recent)
+    last = max(len(p) for p in prompts) + max_new_tokens
+    more = max(page, keep // 8)
+    rows = [len(p) + max_new_tokens for p in prompts]       # of each at most
+    if keep:
+        rows = [min(n, max(keep, len(p)) + more) for n, p in zip(rows, prompts)]
+    max_rows = max(rows)
+    if keep >= max_rows:
+        keep = 0
+    dec = PagedDecoder(model, len(prompts), sum(-(-n // page) for n in rows), page, max_rows, last, keep, recent,
+                       cut=min(max_rows, keep + more) if keep else None)
     g = torch.Generator(device=device)
     if seed is not None:
         g.manual_seed(seed)

@@ -56,7 +56,7 @@ class _Refused:
 
 def _decoder(cache, model):
     dec = object.__new__(PagedDecoder)                       # its constructor captures a step on a GPU
-    dec.model, dec.cache = model, cache
+    dec.model, dec.cache, dec.keep, dec.cut, dec._limit = model, cache, 0, cache.max_rows, [cache.max_rows] * cache.slots
     dec.ids, dec.uniform = torch.zeros(cache.slots, 1, dtype=torch.int64), torch.zeros(cache.slots)
     dec.temperature, dec.top_k = torch.zeros(cache.slots), torch.zeros(cache.slots, dtype=torch.int32)
     dec.top_p, dec.min_p = torch.ones(cache.slots), torch.zeros(cache.slots)
