@@ -4,7 +4,7 @@
 //   index, i stays where the mass ahead of it is at most p times the mass that top-k has left;  min-p: w_i >= min_p;
 //   id = the first i, in the order of the vocabulary, with sum_{j <= i} w_j > u sum_j w_j over what stayed.
 //
-// The result is a whole number that hangs on where sums lie next to a border, so weights are good to 2^-31 of themselves and held as
+// The result is a whole number that hangs on where sums lie next to a border, so weights are good to 2^-30.6 of themselves and held as
 // multiples of 2^-44: sums of up to 2^18 of them are exact, and the same in any order. Some thirty instructions on 32 bits give such a
 // weight (Row::mass); in 64-bit arithmetic it took 2.6 times as long.
 //
@@ -204,10 +204,12 @@ struct Row {
     const int w = width();
     for (int v = from(); v < to(); v += 32 * w) f(v + static_cast<int>(threadIdx.x & 31) * w);
   }
-  // exp((x - max) / T) as a multiple of 2^-44, good to 2^-31 of itself: y = (x - max) 256 log2 e / T as a sum of two numbers, the
-  // whole part n of its 256ths from the table, 2^(f / 256) = 1 + q of the rest by a polynomial, q in 2^-31ths. The largest has exactly
-  // 1. What lies below 2^-45, -inf and NaN shift everything out. Whole-number instructions run at half the rate of the others here: what
-  // can be had from products and sums is.
+  // exp((x - max) / T) as a multiple of 2^-44, good to 2^-30.6 of itself (2^-32 each from the table and from the sum with q, the rest from
+  // the polynomial; of 6 million logits 2^-30.69 at most, one in a thousand beyond 2^-31, 2^-37 on average; the upper half of the product
+  // alone was off by up to 2^-29.4, always downwards): y = (x - max) 256 log2 e / T as a sum of two numbers, the whole part n of its
+  // 256ths from the table, 2^(f / 256) = 1 + q of the rest by a polynomial, q in 2^-31ths. The largest has exactly 1. What lies below
+  // 2^-45, -inf and NaN shift everything out. Whole-number instructions run at half the rate of the others here: what can be had from
+  // products and sums is.
   __device__ __forceinline__ u64 mass(uint32_t key) const {
     const float x = Key<T>::value(key), d = x - top;
     float rest = 0.f;
@@ -222,12 +224,13 @@ struct Row {
     const float f = (y - (t - 12582912.f)) + low;
     const float q = f * fmaf(f, fmaf(f, 3.3083e-9f, 3.66556e-6f), 2.7076062e-3f);       // (ln 2 / 256)^i / i!
     const uint32_t one_q = __float_as_uint(q + 5.859375e-3f) + (0x80000000u - 0x3bc00000u);   // 1.5 2^-8; (1 + q) 2^31
-    const uint32_t w = __umulhi(s->powers[n & 255], one_q);                              // times 2^30
-    const uint32_t shift = 18 + 0x4b4000u - (n >> 8);     // of w 2^32
+    const u64 w = static_cast<u64>(s->powers[n & 255]) * one_q;                          // times 2^62
+    const uint32_t w_hi = static_cast<uint32_t>(w >> 32), w_lo = static_cast<uint32_t>(w);
+    const uint32_t shift = 18 + 0x4b4000u - (n >> 8);
     uint32_t hi, lo, far;
-    asm("shr.u32 %0, %1, %2;" : "=r"(hi) : "r"(w), "r"(shift));             // by 32 and more: 0
-    asm("shr.u32 %0, %1, %2;" : "=r"(far) : "r"(w), "r"(shift - 32));
-    asm("shf.r.clamp.b32 %0, 0, %1, %2;" : "=r"(lo) : "r"(w), "r"(shift));
+    asm("shr.u32 %0, %1, %2;" : "=r"(hi) : "r"(w_hi), "r"(shift));          // by 32 and more: 0
+    asm("shr.u32 %0, %1, %2;" : "=r"(far) : "r"(w_hi), "r"(shift - 32));
+    asm("shf.r.clamp.b32 %0, %1, %2, %3;" : "=r"(lo) : "r"(w_lo), "r"(w_hi), "r"(shift));
     return static_cast<u64>(hi) << 32 | (shift < 32 ? lo : far);
   }
 };
