@@ -170,6 +170,7 @@ class PagedKVCache:
         are those of the steps so far: a prompt's rows come with none."""
         if self.weights is None:
             raise RuntimeError("evict needs a cache with statistics")
+        keep, recent = (min(n, self.width * self.page) for n in (keep, recent))
         lengths = self.lengths
         chosen = range(self.slots) if slots is None else slots
         if slots is not None:                             # the others look as if they were not in use

@@ -1436,6 +1436,9 @@ def _paged(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tens
                       pages, page, width)
 
 
+_INT_MAX = 2 ** 31 - 1                    # ctypes takes the lower 32 bits of a larger number without a word
+
+
 # sizes of workspaces: asked for once per shape and device
 @functools.lru_cache(maxsize=256)
 def _paged_workspace(device: int, *sizes) -> int:
@@ -1545,6 +1548,7 @@ def evict_rows_(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     keep, recent = int(keep), int(recent)
     if keep < 1 or not 0 <= recent <= keep:
         raise RuntimeError("evict_rows_: expected keep >= 1 and 0 <= recent <= keep")
+    keep, recent = min(keep, _INT_MAX), min(recent, _INT_MAX)
     if D % 8:
         raise RuntimeError("pages: the head size must be a multiple of 8")
     if (weights_out is None) != (row_positions_out is None):
@@ -1591,6 +1595,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
         temperatures, temperature = _on(temperature, "temperature", f32, device, (B,)), 1.0
     if isinstance(top_k, tensor):
         top_ks, top_k = _on(top_k, "top_k", torch.int32, device, (B,)), 0
+    else:
+        top_k = max(0, min(top_k, _INT_MAX))
     if isinstance(top_p, tensor):
         top_ps, top_p = _on(top_p, "top_p", f32, device, (B,)), 1.0
     if isinstance(min_p, tensor):
