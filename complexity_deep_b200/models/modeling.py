@@ -182,9 +182,13 @@ class ComplexityModel(nn.Module, GenerationMixin):
                          max_positions: Optional[int] = None, statistics: bool = False) -> PagedKVCache:
         """Cache in pages for sequences of different lengths (see ``PagedDecoder``); max_positions: the longest that a
         sequence gets, its evicted rows included (max_rows unless given)."""
-        c = self.config
-        return PagedKVCache(c.num_hidden_layers, slots, c.num_key_value_heads, c.hidden_size // c.num_attention_heads, pages, page,
-                            max_rows, max_positions or max_rows, self.embed_tokens.weight.device, statistics)
+        c, w = self.config, self.embed_tokens.weight
+        D, group = c.hidden_size // c.num_attention_heads, c.num_attention_heads // c.num_key_value_heads
+        if D not in (64, 128) or group > 16 or w.dtype is not torch.bfloat16:
+            raise RuntimeError("a paged cache needs a bf16 model with heads of 64 or 128 and at most 16 query heads per KV head, not "
+                               f"{str(w.dtype)[6:]}, {D} and {group}")
+        return PagedKVCache(c.num_hidden_layers, slots, c.num_key_value_heads, D, pages, page, max_rows, max_positions or max_rows, w.device,
+                            statistics)
 
     # ------------------------------------------------------------------ utilities
     def num_parameters(self, trainable_only: bool = True) -> int:
