@@ -135,14 +135,17 @@ class PagedKVCache:
         return any(n >= self.max_rows for n in self._length)
 
     def reserve(self) -> None:
-        """A place for the next token in every sequence in use; raises before anything is changed if one has none."""
-        if self.full():
-            raise RuntimeError(f"a sequence has all of its {self.max_rows} rows")
-        if any(n >= 0 and p >= self.max_positions for n, p in zip(self._length, self._position)):
-            raise RuntimeError(f"a sequence is at the last of {self.max_positions} positions")
+        """A place for the next token in every sequence in use.  Raises before anything is changed if one has none, and names those
+        slots: without them (``release``), or with fewer rows in them (``evict``), the others go on."""
+        full = [slot for slot, n in enumerate(self._length) if n >= self.max_rows]
+        if full:
+            raise RuntimeError(f"a sequence has all of its {self.max_rows} rows: slots {full}")
+        last = [slot for slot, (n, p) in enumerate(zip(self._length, self._position)) if n >= 0 and p >= self.max_positions]
+        if last:
+            raise RuntimeError(f"a sequence is at the last of {self.max_positions} positions: slots {last}")
         wanting = [slot for slot, n in enumerate(self._length) if n >= 0 and n == len(self._pages[slot]) * self.page]
         if len(wanting) > len(self._free):
-            raise RuntimeError(f"no page left: {len(wanting)} wanted, {len(self._free)} of {self.pages} free")
+            raise RuntimeError(f"no page left: {len(wanting)} wanted, {len(self._free)} of {self.pages} free: slots {wanting}")
         for slot in wanting:
             self._take(slot, 1)
         if wanting:
