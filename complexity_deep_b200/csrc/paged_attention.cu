@@ -7,7 +7,9 @@
 // the bound, and G only has to stay out of its way. Hence matrix instructions (m16n8k16): the query heads are the 16 rows of one
 // operand. Keys and values are bf16; q (of a step) and p have 32 bits and enter as three bf16 numbers, which hold all 24 of their
 // significant ones. Up to eight heads leave half of the rows free: the first two numbers share a product, the third takes one of its
-// own. More heads take three. A q that comes as bf16 is one number.
+// own. More heads take three. (Of a q that comes as bf16 the others are zero; the third is left out.) us on the device with two numbers and
+// with three: step of 32 x 256 to 2 047 rows, 8 x 2 x 128, weights, 30.3 / 31.5, of 64 x 1 000 to 16 384 224 / 221, of 64 x 250 to 4 000,
+// 4 x 16 x 128, 55.6 / 62.8; without a step the last 52.7 / 54.8, 2 x 32 768 rows of 8 x 2 x 128 49.2 / 49.2.
 //
 // Work is cut into tiles of 64 rows; all tiles of all (sequence, KV head) pairs stand in one line, of which every block takes an equal
 // stretch, whatever the lengths are (a pair's beginning counts as a few tiles: pair_units). A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
@@ -62,7 +64,7 @@ __host__ __device__ constexpr int smem_bytes(int D, bool wide) {
 }
 
 // What beginning a pair costs, in tiles: of the line, these come ahead of the pair's own. Without them a stretch of many short pairs holds
-// all others up. us a step with 0 / 1 / 2 / 4: 64 sequences of 32 to 2 047 rows, 8 x 2 x 128, 56 / 43 / 37 / 37, 16 of them empty 40 / 30 /
+// all others up. us a step with 0 / 1 / 2 / 4 (two numbers of q and p; three add 1 to 7 us to all): 64 sequences of 32 to 2 047 rows, 8 x 2 x 128, 56 / 43 / 37 / 37, 16 of them empty 40 / 30 /
 // 26 / 27, 32 of 256 to 2 047 with weights 31.9 / 30.8 / 30.8 / 31.5, 64 x 1 000 to 16 384 264 / 267 / 266 / 270; of 16 heads, 0 / 1 / 3 / 4 / 5:
 // 55 of 1 197 and eight empty ones, 4 x 16 x 128, 133 / 84 / 62 / 62 / 63, 64 of 250 to 4 000 66 / 61 / 60 / 61 / 62.
 __host__ __device__ constexpr int pair_units(bool wide) { return wide ? 3 : 2; }
