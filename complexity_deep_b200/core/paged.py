@@ -175,10 +175,12 @@ class PagedKVCache:
             raise RuntimeError("evict needs a cache with statistics")
         keep, recent = (min(n, self.width * self.page) for n in (keep, recent))
         lengths = self.lengths
-        chosen = range(self.slots) if slots is None else slots
+        chosen = list(range(self.slots) if slots is None else slots)
+        if not chosen:
+            return
         if slots is not None:                             # the others look as if they were not in use
             these = torch.zeros(self.slots, dtype=torch.bool)
-            these[list(slots)] = True
+            these[chosen] = True
             these = these.to(lengths.device)
             lengths = torch.where(these, lengths, -1)
         ops.evict_rows_(self.k, self.v, self.table, lengths, self.positions, self.weights, self.row_positions, keep, recent)

@@ -41,3 +41,18 @@ def test_cut_back(monkeypatch):
         cache.reserve()
     cache.evict(30, 4, [0])
     _steps(cache, 10)
+
+
+def test_slots_of_a_cut(monkeypatch):
+    """Any iterable of slots, none and one twice; one that there is not changes nothing."""
+    calls = []
+    monkeypatch.setattr(paged.ops, "evict_rows_", lambda *a: calls.append(a[3].tolist()))
+    cache = _cache([40, 41, 42])
+    cache.evict(20, 4, [])
+    with pytest.raises(IndexError):
+        cache.evict(20, 4, [0, 3])
+    assert not calls and cache.lengths.tolist() == [40, 41, 42]
+    cache.evict(20, 4, (slot for slot in (2, 0)))
+    assert calls == [[40, -1, 42]] and cache.lengths.tolist() == [20, 41, 20] == [cache.length(i) for i in range(3)]
+    cache.evict(20, 4, [1, 1])
+    assert cache.lengths.tolist() == [20, 20, 20] and cache.free_pages == 20 - 6
