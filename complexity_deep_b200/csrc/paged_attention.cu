@@ -7,9 +7,9 @@
 // the bound, and G only has to stay out of its way. Hence matrix instructions (m16n8k16): the query heads are the 16 rows of one
 // operand. Keys and values are bf16; q (of a step) and p have 32 bits and enter as three bf16 numbers, which hold all 24 of their
 // significant ones. Up to eight heads leave half of the rows free: the first two numbers share a product, the third takes one of its
-// own. More heads take three. (Of a q that comes as bf16 the others are zero; the third is left out.) us on the device with two numbers and
-// with three: step of 32 x 256 to 2 047 rows, 8 x 2 x 128, weights, 30.3 / 31.5, of 64 x 1 000 to 16 384 224 / 221, of 64 x 250 to 4 000,
-// 4 x 16 x 128, 55.6 / 62.8; without a step the last 52.7 / 54.8, 2 x 32 768 rows of 8 x 2 x 128 49.2 / 49.2.
+// own, in the rows of the second. More heads take three. (Of a q that comes as bf16 the others are zero; the third is left out.) us on the device with two numbers and
+// with three: step of 32 x 256 to 2 047 rows, 8 x 2 x 128, weights, 30.3 / 31.8, of 64 x 1 000 to 16 384 224 / 221, of 64 x 250 to 4 000,
+// 4 x 16 x 128, 55.6 / 65; without a step the last 52.7 / 55.5, 2 x 32 768 rows of 8 x 2 x 128 49.2 / 49.8.
 //
 // Work is cut into tiles of 64 rows; all tiles of all (sequence, KV head) pairs stand in one line, of which every block takes an equal
 // stretch, whatever the lengths are (a pair's beginning counts as a few tiles: pair_units). A stretch that covers a pair writes its output; a pair that is cut leaves a partial sum per
@@ -315,6 +315,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int kStages = stages_of(D, kWide), kHalf = kTile * D * 2;
   constexpr int kHeads = kWide ? 2 : 1;                   // of a lane
   constexpr int kFloats = lane_floats(D, kWide), kPair = pair_units(kWide);
+  // A product adds to its accumulator without rounding: what 24 bits do not hold is cut off, which over hundreds of tiles adds up to
+  // 1e-5 of a sum. Hence, where it costs nothing, sums of 16 rows that are added outside of the products (of 524 288 outputs of 64
+  // sequences of 1 000 to 16 384 rows, 8 x 2 x 128, 159 are rounded otherwise than in 64 bits, 924 without, 472 by sums in 32 bits in
+  // another order; 267 us and 269). Not so in a step, which has a product more (32 x 256 to 2 047 rows 33.4 us and 31.5), for more than eight
+  // heads (64 x 250 to 4 000, 4 x 16 x 128, 58 and 55), and in clusters, where a block has 16 tiles at most. There a tile is cut once or, of
+  // more than eight heads, three times: the third numbers of up to eight go beside the second, whose sums are small.
+  constexpr bool kRound = !kStep && !kWide && !kCluster;
   extern __shared__ unsigned char s_dyn[];
   __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages], s_query, s_query_taken;
   __shared__ int2 s_scan[kThreads / 32];
@@ -585,14 +592,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       place_in_line += take + kPair;
     }
 
-    float m[kHeads], l[kHeads], o[D / 8][4];
+    float m[kHeads], l[kHeads], o[D / 8][kRound ? 2 : 4];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       m[i] = -FLT_MAX;
       l[i] = 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int j = 0; j < D / 8; ++j) {
+#pragma unroll
+      for (int e = 0; e < (kRound ? 2 : 4); ++e) o[j][e] = 0.f;
+    }
 
     for (int t = w.t; t < w.t + take; ++t, ++unit) {
       if (!mbar_wait(&s_full[stage], phase, &s_abort)) atomicMax(a.status, kStatusWaitTimeout);
@@ -625,7 +635,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
           if constexpr (kStep) {
             const uint2 r = s_rest[kHeads * k * 32 + lane], r2 = kWide ? s_rest[(kHeads * k + 1) * 32 + lane] : make_uint2(0, 0);
-            const uint32_t rest[4] = {r.x, r2.x, r.y, r2.y};
+            const uint32_t rest[4] = {kWide ? r.x : 0, kWide ? r2.x : r.x, kWide ? r.y : 0, kWide ? r2.y : r.y};
             mma16816(s[0], rest, kb[0], kb[1]);
             mma16816(s[1], rest, kb[2], kb[3]);
           }
@@ -656,7 +666,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             for (int j = 0; j < D / 8; ++j) {
               o[j][2 * i] *= f;
               o[j][2 * i + 1] *= f;
-              if constexpr (!kWide) {
+              if constexpr (!kWide && !kRound) {
                 o[j][2] *= f;
                 o[j][3] *= f;
               }
@@ -668,8 +678,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             l[i] += x[e];
           }
           uint32_t hi[2], lo[2];
-          split_all(x[0], x[1], hi[0], lo[0], pr[i]);
-          split_all(x[2], x[3], hi[1], lo[1], pr[2 + i]);
+          split_all(x[0], x[1], hi[0], lo[0], pr[kWide ? i : 1]);          // beside the second, whose sums are small
+          split_all(x[2], x[3], hi[1], lo[1], pr[kWide ? 2 + i : 3]);
           if constexpr (kWide) {
             ph[i] = hi[0];
             ph[2 + i] = hi[1];
@@ -699,14 +709,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             vb[2] &= keep0;
             vb[3] &= keep1;
           }
-          mma16816(o[2 * j], ph, vb[0], vb[1]);
-          mma16816(o[2 * j + 1], ph, vb[2], vb[3]);
-          if constexpr (kWide) {
-            mma16816(o[2 * j], pl, vb[0], vb[1]);
-            mma16816(o[2 * j + 1], pl, vb[2], vb[3]);
+          auto add = [&](float (&to)[4], uint32_t b0, uint32_t b1) {
+            mma16816(to, pr, b0, b1);
+            if constexpr (kWide) mma16816(to, pl, b0, b1);
+            mma16816(to, ph, b0, b1);
+          };
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if constexpr (kRound) {
+              float sum[4] = {};
+              add(sum, vb[2 * e], vb[2 * e + 1]);
+              o[2 * j + e][0] += sum[0] + sum[2];
+              o[2 * j + e][1] += sum[1] + sum[3];
+            } else {
+              add(o[2 * j + e], vb[2 * e], vb[2 * e + 1]);
+            }
           }
-          mma16816(o[2 * j], pr, vb[0], vb[1]);
-          mma16816(o[2 * j + 1], pr, vb[2], vb[3]);
         }
       }
       __syncwarp();
@@ -719,9 +737,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     float f[kFloats];
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
-      if constexpr (kWide) {
+      if constexpr (kWide || kRound) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[4 * j + e] = o[j][e];
+        for (int e = 0; e < 2 * kHeads; ++e) f[2 * kHeads * j + e] = o[j][e];
       } else {
         f[2 * j] = o[j][0] + o[j][2];
         f[2 * j + 1] = o[j][1] + o[j][3];
